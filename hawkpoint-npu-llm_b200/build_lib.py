@@ -19,7 +19,7 @@ REPO = PKG.parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libhawkb200.so"
-SOURCES = [CSRC / "hb_engine.cu", CSRC / "hb_batch.cu"]
+SOURCES = [CSRC / "hb_engine.cu", CSRC / "hb_batch.cu", CSRC / "hb_paged.cu"]
 HEADERS = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [REPO / "include" / "hawkb200.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -44,7 +44,7 @@ def build(force=False, verbose_ptxas=False, quiet=False):
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [
-        nvcc_path(), *ARCH, "-O3", "-lineinfo", "-std=c++17",
+        nvcc_path(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "--threads", "4",
         "-Xcompiler", "-fPIC,-O2", "-shared",
         "-I", str(REPO / "include"), "-I", str(CSRC),
         "-o", str(tmp), *map(str, SOURCES),

@@ -146,6 +146,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, Ctrl *
   return mbar_wait_slow(bar, parity, ctrl, limit_ns, where);
 }
 
+// Bounded wait that does not raise on abort (cleanup paths).
+__device__ __forceinline__ void mbar_wait_quiet(uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
+  const uint64_t start = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (globaltimer_ns() - start > limit_ns) return;
+  }
+}
+
 // 16-byte asynchronous copy global -> shared (L2 only, no L1 allocation),
 // grouped with cp_async_commit and completed by cp_async_wait_all.
 __device__ __forceinline__ void cp_async16(void *smem_dst, const void *gmem_src) {

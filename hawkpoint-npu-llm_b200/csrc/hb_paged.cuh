@@ -1,0 +1,311 @@
+// hb_paged.cuh -- what the paged-cache operators share: the page layout, the
+// view of a call's rows, and the division of an attention call's work.
+//
+// A page holds 64 positions of every layer and kv head:
+// [layer][kv head][K | V][head_dim / 64][64 positions][64 dims], two-byte
+// elements, the eight 16-byte blocks of a position's 64 dims stored at
+// block ^ (position & 7).  A [64][64] block is thus 8 KB whose rows of 128
+// bytes are swizzled as a 128-byte-swizzled shared-memory operand wants them:
+// a plain bulk copy of a page's K or V is an MMA operand tile, and its first
+// r positions are its first 128 r bytes.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "hb_attn.cuh"
+
+namespace hb {
+namespace paged {
+
+constexpr int kPage = 64;             // positions a page
+constexpr int kBlockBytes = 8192;     // [64 positions][64 dims]
+constexpr int kMaxEntries = 1024;     // batch entries a call
+
+// The workspace's first bytes: the waits' control block and the operators'
+// sticky status, then what a page operator's first kernel leaves for its
+// second one.
+struct Control {
+  Ctrl ctrl;
+  int status;    // HB_PAGED_* bits, cleared by hb_paged_status
+  int copies;    // entries of the copy list
+  int pad[6];
+};
+static_assert(sizeof(Control) == 64, "control block");
+
+// A pool as the kernels see it.
+struct Pool {
+  uint8_t *pages;
+  int64_t page_stride;   // bytes from page to page
+  int n_pages, kv_heads, width, n_slots;
+  int *table, *refs, *lengths;
+  Control *control;
+};
+
+// A call's rows: entry b is slot slots[b] with rows row_start[b] ..
+// row_start[b + 1].
+struct Batch {
+  const int *slots, *row_start;
+  int entries, rows;
+};
+
+struct Entry {
+  int row0, n, length, slot;   // slot -1: none (its rows see nothing)
+};
+
+// Entry b with every index held inside its array.
+__device__ __forceinline__ Entry entry_of(const Pool &P, const Batch &B, int b) {
+  Entry e;
+  e.row0 = min(max(B.row_start[b], 0), B.rows);
+  e.n = min(max(B.row_start[b + 1], e.row0), B.rows) - e.row0;
+  e.slot = B.slots[b];
+  if (e.slot < 0 || e.slot >= P.n_slots) e.slot = -1;
+  e.length = e.slot < 0 ? 0 : max(P.lengths[e.slot], 0);
+  return e;
+}
+
+// ---- division of an attention call --------------------------------------------
+// The rows of an entry and the q heads of a kv head's group are packed into
+// tiles of `tile` rows: packed row r is row r / group, head r % group.  A
+// tile's work is the blocks of `block` positions that any of its rows sees
+// (one at least, so that a tile without any is still written).  The blocks of
+// all tiles, entry by entry, head by head, are one line that the thread
+// blocks cut into equal pieces, so ragged lengths leave none idle; a tile cut
+// by a border is joined from its parts.
+struct Shape {
+  int group, width, window, tile, block;
+};
+
+struct Span {
+  int lo, hi;   // blocks [lo, hi) of positions; hi <= lo: none
+};
+
+__device__ __forceinline__ Span tile_span(const Shape &S, const Entry &e, int t) {
+  const int packed = e.n * S.group;
+  const int i0 = t * S.tile / S.group, i1 = (min(packed, (t + 1) * S.tile) - 1) / S.group;
+  const int last = e.length - e.n + i1, first = e.length - e.n + i0;
+  Span s;
+  s.hi = last < 0 ? 0 : min(last / S.block, (S.width * kPage - 1) / S.block) + 1;
+  s.lo = S.window > 0 ? max(0, first - S.window + 1) / S.block : 0;
+  return s;
+}
+__device__ __forceinline__ int tile_units(const Shape &S, const Entry &e, int t) {
+  const Span s = tile_span(S, e, t);
+  return max(1, s.hi - s.lo);
+}
+__device__ __forceinline__ int tiles_of(const Shape &S, const Entry &e) { return (e.n * S.group + S.tile - 1) / S.tile; }
+
+// The line of a call: prefix[b] = units before entry b (shared memory,
+// kMaxEntries + 1), filled by all threads of the block.  `take(entry)` says
+// whether this kernel takes an entry's rows.
+template <class Take>
+__device__ __forceinline__ void fill_prefix(const Pool &P, const Batch &B, const Shape &S, int64_t *prefix,
+                                            const Take &take) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  for (int b = warp; b < B.entries; b += warps) {
+    const Entry e = entry_of(P, B, b);
+    int64_t u = 0;
+    if (take(e))
+      for (int t = lane; t < tiles_of(S, e); t += 32) u += tile_units(S, e, t);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    if (lane == 0) prefix[b + 1] = u * P.kv_heads;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < B.entries; b0 += 32) {
+      const int b = b0 + lane;
+      int64_t v = b < B.entries ? prefix[b + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += w;
+      }
+      if (b < B.entries) prefix[b + 1] = base + v;
+      base += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+  }
+  __syncthreads();
+}
+
+// A walk over the tiles of one piece [u, end) of the line.
+struct Walk {
+  int64_t u, end;        // units left
+  int64_t tile_u;        // first unit of the current tile
+  int b, head, t, units;
+  Entry e;
+  Span span;
+
+  // positions on the tile that holds unit u; false when the piece is done
+  __device__ __forceinline__ bool start(const Pool &P, const Batch &B, const Shape &S, const int64_t *prefix) {
+    if (u >= end) return false;
+    int lo = 0, hi = B.entries - 1;
+    while (lo < hi) {  // the last entry whose prefix is <= u and that has units
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid + 1] > u) hi = mid; else lo = mid + 1;
+    }
+    b = lo;
+    e = entry_of(P, B, b);
+    const int64_t per = (prefix[b + 1] - prefix[b]) / P.kv_heads;
+    const int64_t rem = u - prefix[b];
+    head = static_cast<int>(rem / per);
+    tile_u = prefix[b] + head * per;
+    t = 0;
+    units = tile_units(S, e, 0);
+    while (tile_u + units <= u) {
+      tile_u += units;
+      units = tile_units(S, e, ++t);
+    }
+    span = tile_span(S, e, t);
+    return true;
+  }
+  // blocks of the tile that lie in the piece: [first, first + count)
+  __device__ __forceinline__ int first() const { return span.lo + static_cast<int>(u - tile_u); }
+  __device__ __forceinline__ int count() const {
+    return static_cast<int>(min(end, tile_u + units) - u);
+  }
+  __device__ __forceinline__ bool next(const Pool &P, const Batch &B, const Shape &S, const int64_t *prefix) {
+    u = tile_u + units;
+    if (u >= end) return false;
+    if (t + 1 < tiles_of(S, e)) {
+      tile_u = u;
+      units = tile_units(S, e, ++t);
+      span = tile_span(S, e, t);
+      return true;
+    }
+    if (head + 1 < P.kv_heads) {
+      ++head;
+      t = 0;
+      tile_u = u;
+      units = tile_units(S, e, 0);
+      span = tile_span(S, e, 0);
+      return true;
+    }
+    return start(P, B, S, prefix);
+  }
+};
+
+// Piece c of `pieces` equal pieces of [0, total).
+__device__ __forceinline__ int64_t piece_begin(int64_t total, int pieces, int c) {
+  return total * c / pieces;
+}
+// The piece that holds unit u.
+__device__ __forceinline__ int piece_of(int64_t total, int pieces, int64_t u) {
+  int c = static_cast<int>(u * pieces / total);
+  while (c + 1 < pieces && piece_begin(total, pieces, c + 1) <= u) ++c;
+  while (c > 0 && piece_begin(total, pieces, c) > u) --c;
+  return c;
+}
+
+// ---- elements -------------------------------------------------------------------
+template <class T>
+struct Elem;
+template <>
+struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ float lo(uint32_t u) { return bf_lo(u); }
+  static __device__ __forceinline__ float hi(uint32_t u) { return bf_hi(u); }
+  static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+  }
+};
+template <>
+struct Elem<__half> {
+  static __device__ __forceinline__ float lo(uint32_t u) { return __half2float(__ushort_as_half(u & 0xffffu)); }
+  static __device__ __forceinline__ float hi(uint32_t u) { return __half2float(__ushort_as_half(u >> 16)); }
+  static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+  }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What an attention kernel gets.
+struct Attend {
+  Pool pool;
+  Batch batch;
+  int64_t layer_off, head_bytes;   // bytes: of the layer in a page, of a kv head's K and V
+  const void *q;
+  int64_t q_row, q_head;           // strides in elements
+  void *out;
+  int64_t o_row, o_head;
+  float *lse;                      // [rows][q_heads], or NULL
+  int q_heads;
+  Shape shape;
+  float scale, scale_log2;         // of the scores; times log2(e)
+  int q_vec, o_vec;                // q rows / out rows are 16-byte aligned
+  float *parts;                    // joined tiles: per piece two parts
+  int *arrived;                    // per piece, zero between launches
+  uint64_t limit_ns;
+};
+
+__device__ __forceinline__ const uint8_t *kv_block(const Attend &A, int page, int head) {
+  return A.pool.pages + static_cast<int64_t>(page) * A.pool.page_stride + A.layer_off + head * A.head_bytes;
+}
+
+// Page `j` of a slot, -1 where none is mapped.
+__device__ __forceinline__ int page_of(const Pool &P, int slot, int j) {
+  if (slot < 0 || j < 0 || j >= P.width) return -1;
+  const int pg = P.table[static_cast<int64_t>(slot) * P.width + j];
+  return pg >= 0 && pg < P.n_pages ? pg : -1;
+}
+
+// One output row by one warp from the positions it sees alone, in FP32.  The
+// tiled kernels multiply hidden positions by weight zero, which an infinity or
+// NaN among their V would turn into NaN; a row that comes out not finite is
+// done again here, so that what a row does not see never reaches it.
+template <int D, class T>
+__device__ __noinline__ void row_alone(const Attend &A, const Entry &e, int head, int i, int g) {
+  using E = Elem<T>;
+  constexpr int kPer = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int qh = head * A.shape.group + g, row = e.row0 + i, p = e.length - e.n + i;
+  const T *q = static_cast<const T *>(A.q) + row * A.q_row + qh * A.q_head;
+  float qf[kPer], o[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    qf[k] = E::get(q[lane + 32 * k]);
+    o[k] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  const int lo = A.shape.window > 0 ? max(0, p - A.shape.window + 1) : 0;
+  const int hi = min(p, A.shape.width * kPage - 1);
+  for (int j = lo; j <= hi; ++j) {
+    const int pg = page_of(A.pool, e.slot, j >> 6);
+    if (pg < 0) continue;
+    const uint8_t *kb = kv_block(A, pg, head);
+    float dot = 0.f, v[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int d = lane + 32 * k;
+      const int off = (d >> 6) * kBlockBytes + kv_off(j & 63, (d & 63) >> 3) + (d & 7) * 2;
+      dot = fmaf(qf[k], E::get(*reinterpret_cast<const T *>(kb + off)), dot);
+      v[k] = E::get(*reinterpret_cast<const T *>(kb + D / 64 * kBlockBytes + off));
+    }
+    const float s = warp_sum(dot);
+    const float nm = fmaxf(m, s), use = nm == -INFINITY ? 0.f : nm;
+    const float a = exp2_approx((m - use) * A.scale_log2), w = exp2_approx((s - use) * A.scale_log2);
+    m = nm;
+    l = fmaf(l, a, w);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) o[k] = fmaf(w, v[k], o[k] * a);
+  }
+  T *out = static_cast<T *>(A.out) + row * A.o_row + qh * A.o_head;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) out[lane + 32 * k] = E::put(l == 0.f ? 0.f : o[k] / l);
+}
+
+}  // namespace paged
+}  // namespace hb

@@ -213,14 +213,6 @@ enum : int {
   kEpiLogits = 4,  // FP32 logits (optional) and each row's maximum over the tile (np.argmax order)
 };
 
-// Bounded wait that does not raise on abort (cleanup paths).
-__device__ __forceinline__ void mbar_wait_quiet(uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
-  const uint64_t start = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer_ns() - start > limit_ns) return;
-  }
-}
-
 // Row n of `out` (packed row-group layout) = bf16((x * inv_rms) * gamma) of
 // the BF16 row x (cpu_backend.py:71-76); one warp, lane l taking 16-byte
 // chunks l, l + 32, ... (held in registers for rows of up to 1024 values).

@@ -34,6 +34,12 @@ HB_GEMV_OUT_F32 = 1
 HB_GEMV_OUT_NONE = 2
 HB_GEMV_ARGMAX = 4
 
+HB_ELEM_BF16 = 0
+HB_ELEM_FP16 = 1
+HB_PAGED_EXHAUSTED = 1
+HB_PAGED_BAD_INDEX = 2
+HB_PAGED_UNMAPPED = 4
+
 ABI_VERSION = 1
 
 
@@ -83,6 +89,75 @@ class HbSampling(ctypes.Structure):
         ("bias_tokens", ctypes.POINTER(ctypes.c_int32)),
         ("bias_values", ctypes.POINTER(ctypes.c_float)),
         ("uniform", ctypes.c_double),
+    ]
+
+
+class HbPagePool(ctypes.Structure):
+    """hb_page_pool: a page pool and its books, all on the device."""
+
+    _fields_ = [
+        ("pages_dev", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("n_pages", ctypes.c_int32),
+        ("layers", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("element", ctypes.c_int32),
+        ("n_slots", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+        ("table_dev", ctypes.c_void_p),
+        ("refs_dev", ctypes.c_void_p),
+        ("lengths_dev", ctypes.c_void_p),
+        ("workspace_dev", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class HbPagedRows(ctypes.Structure):
+    """hb_paged_rows: the rows of a paged call."""
+
+    _fields_ = [
+        ("slots_dev", ctypes.c_void_p),
+        ("row_start_dev", ctypes.c_void_p),
+        ("entries", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class HbPagedQuery(ctypes.Structure):
+    """hb_paged_query: what hb_paged_attend reads and writes beside the pool."""
+
+    _fields_ = [
+        ("q_dev", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("out_dev", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("lse_dev", ctypes.c_void_p),
+        ("q_heads", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class HbPagedNew(ctypes.Structure):
+    """hb_paged_new: the rows hb_paged_append rotates and stores."""
+
+    _fields_ = [
+        ("qkv_dev", ctypes.c_void_p),
+        ("qkv_row_stride", ctypes.c_int64),
+        ("q_dev", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("cos_dev", ctypes.c_void_p),
+        ("sin_dev", ctypes.c_void_p),
+        ("rope_positions", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
     ]
 
 
@@ -136,6 +211,15 @@ SIGNATURES = {
     "hb_tc_gemm_status": (_I, [_P, _P]),
     "hb_step_rows": (_I, [_P, _I, _I32P, _I32P, _I32P, _I, _I32P, _I32P, _FP]),
     "hb_prefill_tc": (_I, [_P, _I, _I32P, _I, _I, _FP, _I32P]),
+    "hb_paged_workspace_bytes": (ctypes.c_size_t, [_P]),
+    "hb_paged_status": (_I, [_P, _I32P, _P]),
+    "hb_paged_attend": (_I, [_P, _I, _P, _P, _P]),
+    "hb_paged_append": (_I, [_P, _I, _P, _P, _P]),
+    "hb_pages_reserve": (_I, [_P, _I, _P, _P, _P]),
+    "hb_pages_fork": (_I, [_P, _I, _P, _P, _P, _P]),
+    "hb_pages_free": (_I, [_P, _I, _P, _P]),
+    "hb_pages_compact": (_I, [_P, _P, _P]),
+    "hb_pages_copy": (_I, [_P, _I, _P, _P, _P, _I, _P]),
     "hb_library_error": (ctypes.c_char_p, []),
     "hb_device_sm_count": (_I, [_I]),
 }

@@ -1,0 +1,246 @@
+"""A paged K/V cache on the device, and the operators on it.
+
+``PagedKVCache`` holds a pool of 64-position pages with its books (page table,
+reference counts, lengths) in device memory and calls the paged operators of
+libhawkb200.so (include/hawkb200.h) on torch tensors, on torch's current
+stream: nothing here waits for the GPU or copies to the host, except
+``status``.  The reference keeps one contiguous 64-position cache per process
+(npu_llm/runtime/qwen_engine.py:65-94); the engine's own paged cache
+(``B200DecoderEngine(context=...)``) keeps its books on the host.
+
+A step of a serving loop, per layer the two calls in the middle::
+
+    cache.reserve(slots, counts)                  # room for the new rows
+    q = cache.append(layer, qkv, slots, row_start, max_rows, cos, sin)
+    o = cache.attend(layer, q, slots, row_start, max_rows)
+    cache.fork(src, dst, counts); cache.free(done); cache.compact()
+
+Entry b of a call is slot ``slots[b]`` with rows ``row_start[b] ..
+row_start[b + 1]``; its row i of n stands at position ``lengths[slot] - n + i``.
+All index lists are int32 device tensors.  Pages are laid out
+``[layer][kv head][K | V][head_dim / 64][64 positions][64 dims]`` with the
+16-byte blocks of a position's 64 dims stored at block ^ (position & 7);
+``rows`` gives a slot's K and V in plain order.
+
+Calls on one cache share its workspace: run them on one stream, or order the
+streams with events.
+"""
+
+import ctypes
+import math
+
+from runtime import hb_lib
+
+PAGE = 64
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+class PagedKVCache:
+    """A pool of ``n_pages`` pages and its books for ``n_slots`` sequences of
+    up to ``max_context`` positions (rounded up to whole pages)."""
+
+    def __init__(self, layers, kv_heads, head_dim, n_pages, n_slots, max_context, dtype=None, device=None):
+        torch = _torch()
+        dtype = torch.bfloat16 if dtype is None else dtype
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        if min(layers, kv_heads, n_pages, n_slots, max_context) < 1:
+            raise ValueError("layers, kv_heads, n_pages, n_slots and max_context must be positive")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim {head_dim}: must be 64 or 128")
+        ints = dict(dtype=torch.int32, device=device)
+        self._bind(torch.zeros((n_pages, layers, kv_heads, 2, head_dim // 64, PAGE, 64), dtype=dtype, device=device),
+                   torch.full((n_slots, -(-max_context // PAGE)), -1, **ints), torch.zeros(n_pages, **ints),
+                   torch.zeros(n_slots, **ints))
+
+    @classmethod
+    def wrap(cls, pool, table, refs, lengths):
+        """A cache over the caller's tensors: ``pool`` [pages, layers, kv
+        heads, 2, head_dim / 64, 64, 64] (pages may lie apart, a page's
+        elements together), ``table`` int32 [slots, pages a slot], ``refs`` int32
+        [pages], ``lengths`` int32 [slots]."""
+        cache = cls.__new__(cls)
+        cache._bind(pool, table, refs, lengths)
+        return cache
+
+    def _bind(self, pool, table, refs, lengths):
+        torch = _torch()
+        elements = {torch.bfloat16: hb_lib.HB_ELEM_BF16, torch.float16: hb_lib.HB_ELEM_FP16}
+        if pool.dtype not in elements:
+            raise ValueError(f"pool of {pool.dtype}: must be bfloat16 or float16")
+        if pool.dim() != 7 or pool.shape[3] != 2 or tuple(pool.shape[5:]) != (PAGE, 64) or pool.shape[4] not in (1, 2):
+            raise ValueError(f"pool of shape {tuple(pool.shape)}: must be [pages, layers, kv heads, 2, head_dim / 64, 64, 64]")
+        if pool.shape[0] < 1 or not pool[0].is_contiguous():
+            raise ValueError("a page's elements must be contiguous")
+        n_pages, layers, kv_heads = (int(x) for x in pool.shape[:3])
+        for name, t, shape in (("table", table, None), ("refs", refs, (n_pages,)), ("lengths", lengths, (table.shape[0],))):
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.device != pool.device:
+                raise ValueError(f"{name} must be a contiguous int32 tensor on the pool's device")
+            if shape is not None and tuple(t.shape) != shape:
+                raise ValueError(f"{name} of shape {tuple(t.shape)}: must be {shape}")
+        if table.dim() != 2:
+            raise ValueError("table must have a row a slot")
+        self._lib = hb_lib.load()
+        self.pool, self.table, self.refs, self.lengths = pool, table, refs, lengths
+        self.device, self.dtype = pool.device, pool.dtype
+        self.layers, self.kv_heads, self.head_dim = layers, kv_heads, 64 * int(pool.shape[4])
+        p = self._desc = hb_lib.HbPagePool(
+            pages_dev=pool.data_ptr(), page_stride=pool.stride(0) * 2, n_pages=n_pages, layers=layers,
+            kv_heads=kv_heads, head_dim=self.head_dim, element=elements[pool.dtype], n_slots=int(table.shape[0]),
+            table_width=int(table.shape[1]), table_dev=table.data_ptr(), refs_dev=refs.data_ptr(),
+            lengths_dev=lengths.data_ptr())
+        if n_pages == 1:
+            p.page_stride = pool[0].numel() * 2
+        self._pool = ctypes.byref(p)
+        need = self._lib.hb_paged_workspace_bytes(self._pool)
+        if need == 0:
+            hb_lib.check(hb_lib.HB_ERR_INVALID_ARG)
+        self._workspace = torch.zeros(need, dtype=torch.uint8, device=pool.device)
+        p.workspace_dev, p.workspace_bytes = self._workspace.data_ptr(), need
+        self._index = pool.device.index if pool.device.index is not None else torch.cuda.current_device()
+
+    # -- helpers -----------------------------------------------------------------
+    def _stream(self):
+        return _torch().cuda.current_stream(self._index).cuda_stream
+
+    def _call(self, fn, *args):
+        torch = _torch()
+        if torch.cuda.current_device() == self._index:
+            rc = fn(self._pool, *args, self._stream())
+        else:
+            with torch.cuda.device(self._index):
+                rc = fn(self._pool, *args, self._stream())
+        if rc:
+            hb_lib.check(rc)
+
+    def _list(self, name, t, n=None):
+        if t.dtype != _torch().int32 or t.dim() != 1 or not t.is_contiguous() or t.device != self.device:
+            raise ValueError(f"{name} must be a contiguous one-dimensional int32 tensor on the cache's device")
+        if n is not None and t.shape[0] != n:
+            raise ValueError(f"{name} has {t.shape[0]} entries, not {n}")
+        return t.data_ptr()
+
+    def _rows(self, slots, row_start, rows, max_rows):
+        entries = slots.shape[0]
+        if max_rows < 0 or (entries == 0 and rows > 0):
+            raise ValueError("max_rows must not be negative, and rows need an entry")
+        return hb_lib.HbPagedRows(self._list("slots", slots), self._list("row_start", row_start, entries + 1), entries,
+                                  rows, min(int(max_rows), rows), 0)
+
+    def _heads(self, name, t, rows=None):
+        if t.dim() != 3 or t.dtype != self.dtype or t.device != self.device or t.shape[2] != self.head_dim or (
+                t.stride(2) != 1):
+            raise ValueError(f"{name} must be [rows, heads, {self.head_dim}] of {self.dtype} on the cache's device, "
+                             "its last dimension contiguous")
+        if rows is not None and tuple(t.shape[:2]) != rows:
+            raise ValueError(f"{name} of shape {tuple(t.shape)}: must be {rows + (self.head_dim,)}")
+        return t
+
+    # -- rows ----------------------------------------------------------------------
+    def append(self, layer, qkv, slots, row_start, max_rows, cos, sin, out=None):
+        """Rotates the rows' q and k at their positions and stores k and v in
+        the slots' pages (``reserve`` has mapped them).  ``qkv`` [rows, (q
+        heads + 2 kv heads) * head_dim]; ``cos`` / ``sin`` float32 [positions,
+        head_dim / 2].  Returns the rotated q [rows, q heads, head_dim]."""
+        torch = _torch()
+        d = self.head_dim
+        if qkv.dim() != 2 or qkv.dtype != self.dtype or qkv.device != self.device or qkv.stride(1) != 1 or qkv.shape[1] % d:
+            raise ValueError(f"qkv must be [rows, heads * {d}] of {self.dtype} on the cache's device, its last "
+                             "dimension contiguous")
+        rows, q_heads = int(qkv.shape[0]), int(qkv.shape[1]) // d - 2 * self.kv_heads
+        if q_heads < 0:
+            raise ValueError(f"qkv has fewer heads than the {2 * self.kv_heads} of k and v")
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] * 2 != d or not t.is_contiguous() or (
+                    t.device != self.device):
+                raise ValueError(f"{name} must be a contiguous float32 [positions, {d // 2}] on the cache's device")
+        if cos.shape != sin.shape:
+            raise ValueError("cos and sin must have the same shape")
+        if out is None:
+            out = torch.empty((rows, q_heads, d), dtype=self.dtype, device=self.device)
+        else:
+            self._heads("out", out, (rows, q_heads))
+        r = self._rows(slots, row_start, rows, max_rows)
+        n = hb_lib.HbPagedNew(qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), out.stride(1),
+                              cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_heads)
+        self._call(self._lib.hb_paged_append, layer, ctypes.byref(r), ctypes.byref(n))
+        return out
+
+    def attend(self, layer, q, slots, row_start, max_rows, scale=None, window=0, out=None, lse=False):
+        """Attention of the rows' ``q`` [rows, q heads, head_dim] over their
+        slots' positions up to each row's own (with ``window``: the last
+        ``window`` of them); ``scale`` defaults to 1 / sqrt(head_dim).  Returns
+        the output in q's shape; with ``lse`` also float32 [rows, q heads], the
+        log of the sum of exp(scores).  Rows that see nothing give 0 and -inf."""
+        torch = _torch()
+        self._heads("q", q)
+        rows, q_heads = int(q.shape[0]), int(q.shape[1])
+        if out is None:
+            out = torch.empty((rows, q_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        else:
+            self._heads("out", out, (rows, q_heads))
+        sums = torch.empty((rows, q_heads), dtype=torch.float32, device=self.device) if lse else None
+        r = self._rows(slots, row_start, rows, max_rows)
+        a = hb_lib.HbPagedQuery(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                                sums.data_ptr() if lse else None, q_heads, window,
+                                1.0 / math.sqrt(self.head_dim) if scale is None else scale, 0)
+        self._call(self._lib.hb_paged_attend, layer, ctypes.byref(r), ctypes.byref(a))
+        return (out, sums) if lse else out
+
+    # -- pages -----------------------------------------------------------------------
+    def reserve(self, slots, counts):
+        """Room for ``counts[b]`` more positions of ``slots[b]``: lengths grow,
+        missing pages are mapped (the lowest free ones), shared pages that
+        will be written become the slot's own.  All or nothing (``status``)."""
+        n = slots.shape[0]
+        self._call(self._lib.hb_pages_reserve, n, self._list("slots", slots), self._list("counts", counts, n))
+
+    def fork(self, src, dst, counts):
+        """Slot ``dst[b]`` becomes the first ``counts[b]`` positions of
+        ``src[b]`` as it was before the call; whole pages are shared."""
+        n = src.shape[0]
+        self._call(self._lib.hb_pages_fork, n, self._list("src", src), self._list("dst", dst, n),
+                   self._list("counts", counts, n))
+
+    def free(self, slots):
+        """The slots' pages go back to the pool; their lengths become 0."""
+        self._call(self._lib.hb_pages_free, slots.shape[0], self._list("slots", slots))
+
+    def compact(self):
+        """Moves the pages in use to the pool's lowest indices; returns each
+        page's new index, int32 [pages], -1 for a free one."""
+        page_map = _torch().empty_like(self.refs)
+        self._call(self._lib.hb_pages_compact, page_map.data_ptr())
+        return page_map
+
+    def copy_pages(self, src, dst, to=None):
+        """Copies whole pages ``src[i]`` to ``dst[i]`` of this pool, or of the
+        cache ``to`` of the same layout.  No books change."""
+        n = src.shape[0]
+        if to is not None and (to.pool.shape[1:] != self.pool.shape[1:] or to.dtype != self.dtype
+                               or to.device != self.device or to._desc.page_stride != self._desc.page_stride):
+            raise ValueError("the destination's pages must have this cache's layout")
+        self._call(self._lib.hb_pages_copy, n, self._list("src", src), self._list("dst", dst, n),
+                   to.pool.data_ptr() if to is not None else None, to._desc.n_pages if to is not None else 0)
+
+    def status(self):
+        """Waits for the stream and raises what the calls since the last
+        status met on the device: ``HbTimeout``, or ``HbError`` for an
+        exhausted pool, an index out of range or a row without a page."""
+        self._call(lambda pool, stream: self._lib.hb_paged_status(pool, None, stream))
+
+    def rows(self, layer, slot):
+        """K and V of a slot's positions in plain order, [2, kv heads, length,
+        head_dim] (diagnostics: reads the table on the host)."""
+        torch = _torch()
+        length = int(self.lengths[slot])
+        pages = self.table[slot, : -(-length // PAGE)].long()
+        x = self.pool[pages, layer].view(len(pages), self.kv_heads, 2, -1, PAGE, 8, 8)
+        at = torch.arange(PAGE, device=self.device)[:, None]
+        x = x[..., at, torch.arange(8, device=self.device)[None, :] ^ (at & 7), :]
+        x = x.permute(2, 1, 0, 4, 3, 5, 6).reshape(2, self.kv_heads, -1, self.head_dim)
+        return x[:, :, :length]

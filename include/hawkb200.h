@@ -345,6 +345,124 @@ int hb_step_rows(hb_engine *engine, int n, const int32_t *slots, const int32_t *
 int hb_prefill_tc(hb_engine *engine, int slot, const int32_t *ids, int n, int start_pos, float *last_logits,
                   int32_t *argmax_out);
 
+/* ---- paged K/V cache operators (new in this build) -----------------------------
+ * A page pool whose books live on the device: RoPE and append of new rows,
+ * attention of new rows over their slots' pages, and the page operators
+ * (reserve, fork, free, compact, copy).  Every call is asynchronous on
+ * `stream`, allocates nothing, reads its lengths, tables and row lists on the
+ * device and can be captured in a CUDA graph, so a serving loop runs without
+ * host round trips.  The reference keeps one contiguous 64-position cache on
+ * the host (npu_llm/runtime/qwen_engine.py:65-94, cpu_backend.py:95-129).
+ *
+ * A page holds 64 positions of every layer and kv head, in the layout of the
+ * engine's paged cache: [layer][kv head][K | V][head_dim / 64][64
+ * positions][64 dims] of two-byte elements, the eight 16-byte blocks of a
+ * position's 64 dims stored at block ^ (position & 7).
+ *
+ * The caller owns all memory and orders the calls on one pool (they share its
+ * workspace): one stream, or events between streams.  What only the device
+ * can see -- an exhausted pool, an index out of range, a row without a page --
+ * is not an error of the call: it does nothing there, sets a bit in the
+ * workspace, and hb_paged_status reports it. */
+enum { HB_ELEM_BF16 = 0, HB_ELEM_FP16 = 1 };
+enum {
+  HB_PAGED_EXHAUSTED = 1,   /* reserve / fork found too few free pages and changed nothing */
+  HB_PAGED_BAD_INDEX = 2,   /* a slot, page, position, count or length out of range */
+  HB_PAGED_UNMAPPED = 4     /* append: a row's position has no page; its K / V were dropped */
+};
+
+typedef struct hb_page_pool {
+  void *pages_dev;          /* n_pages pages, page_stride bytes apart, 128-byte aligned */
+  int64_t page_stride;      /* at least a page's bytes, a multiple of 128 */
+  int32_t n_pages, layers, kv_heads;
+  int32_t head_dim;         /* 64 or 128 */
+  int32_t element;          /* HB_ELEM_* */
+  int32_t n_slots, table_width;
+  int32_t reserved0;
+  int32_t *table_dev;       /* [n_slots][table_width]: page of each 64 positions, -1 none */
+  int32_t *refs_dev;        /* [n_pages]: slots that hold the page */
+  int32_t *lengths_dev;     /* [n_slots]: positions, rows about to be appended included */
+  void *workspace_dev;      /* hb_paged_workspace_bytes, 256-byte aligned, zero before its first use */
+  uint64_t workspace_bytes;
+} hb_page_pool;
+
+/* The rows of a call: entry b is slot slots_dev[b] with rows row_start_dev[b]
+ * .. row_start_dev[b + 1] (ascending from 0; entries + 1 values); row i of its n stands at
+ * position lengths[slot] - n + i.  At most 1024 entries.  max_rows: the most
+ * rows of an entry (an upper bound; it chooses kernels, never results). */
+typedef struct hb_paged_rows {
+  const int32_t *slots_dev, *row_start_dev;
+  int32_t entries, rows, max_rows, reserved0;
+} hb_paged_rows;
+
+typedef struct hb_paged_query {
+  const void *q_dev;        /* [rows][q_heads][head_dim], strides in elements, dims contiguous */
+  int64_t q_row_stride, q_head_stride;
+  void *out_dev;            /* the same shape */
+  int64_t out_row_stride, out_head_stride;
+  float *lse_dev;           /* [rows][q_heads] log of the sum of exp(scores), or NULL */
+  int32_t q_heads;          /* a multiple of kv_heads: q head h reads kv head h / (q_heads / kv_heads) */
+  int32_t window;           /* 0, or: a row sees the last `window` positions up to its own */
+  float scale;              /* of q.k, positive */
+  int32_t reserved0;
+} hb_paged_query;
+
+typedef struct hb_paged_new {
+  const void *qkv_dev;      /* [rows][(q_heads + 2 kv_heads) * head_dim]: q, k and v heads of a row */
+  int64_t qkv_row_stride;   /* elements */
+  void *q_dev;              /* [rows][q_heads][head_dim]: the rotated q */
+  int64_t q_row_stride, q_head_stride;
+  const float *cos_dev, *sin_dev;   /* [rope_positions][head_dim / 2], 16-byte aligned */
+  int32_t rope_positions, q_heads;
+} hb_paged_new;
+
+/* Bytes of a pool's workspace (0: the shape is not one these calls take;
+ * pointers are not read). */
+size_t hb_paged_workspace_bytes(const hb_page_pool *pool);
+/* Waits for `stream`, reports what the calls since the last status met
+ * (HB_ERR_STATE with the bits in *status; HB_ERR_DEVICE_TIMEOUT when a device
+ * wait gave up) and clears it.  status may be NULL. */
+int hb_paged_status(const hb_page_pool *pool, int32_t *status, void *stream);
+/* out = softmax(scale q.K + mask) V over one layer's pages: a row sees the
+ * mapped positions up to its own, with a window the last `window` of them.  A
+ * row that sees none gives zeros and an lse of -infinity.  Positions that a row does
+ * not see never reach it, whatever they hold.  Scores, sums and the running
+ * maximum are FP32; the weights are rounded to the element type for the
+ * product with V where an entry has more than 16 rows of one kv head, else
+ * kept to twice its bits; out is rounded once. */
+int hb_paged_attend(const hb_page_pool *pool, int layer, const hb_paged_rows *rows, const hb_paged_query *query,
+                    void *stream);
+/* Rotates the rows' q and k (rotate-half RoPE with each row's position, the
+ * persistent decoder's rounding), writes q, and k and v into one layer of the
+ * slots' pages (which hb_pages_reserve mapped). */
+int hb_paged_append(const hb_page_pool *pool, int layer, const hb_paged_rows *rows, const hb_paged_new *rows_new,
+                    void *stream);
+/* Room for counts_dev[b] more positions of slot slots_dev[b] (distinct slots):
+ * lengths grow, missing pages are the lowest free ones in entry order, and a
+ * page that other slots share is made the slot's own before it is written
+ * (its positions below the old length copied).  All or nothing. */
+int hb_pages_reserve(const hb_page_pool *pool, int n, const int32_t *slots_dev, const int32_t *counts_dev,
+                     void *stream);
+/* Slot dst_dev[b] becomes the first counts_dev[b] positions of slot src_dev[b],
+ * all sources as they were before the call (a beam's permutation is one call;
+ * destinations distinct): whole pages are shared, a partial last page is
+ * copied to the lowest free pages in entry order.  What the destinations held
+ * is given up; those pages are free from the next call on.  All or nothing. */
+int hb_pages_fork(const hb_page_pool *pool, int n, const int32_t *src_dev, const int32_t *dst_dev,
+                  const int32_t *counts_dev, void *stream);
+/* The slots' pages go back (a shared page when its last slot gives it up);
+ * table entries become -1, lengths 0. */
+int hb_pages_free(const hb_page_pool *pool, int n, const int32_t *slots_dev, void *stream);
+/* Closes the pool's gaps: with L pages in use, the k-th page in use at index L
+ * or above moves to the k-th free index below L; table and refs follow.
+ * map_dev [n_pages]: each page's new index, -1 for a free one. */
+int hb_pages_compact(const hb_page_pool *pool, int32_t *map_dev, void *stream);
+/* Copies whole pages src_dev[i] -> dst_dev[i] of this pool, or of
+ * dst_pages_dev (dst_n_pages pages of the same layout and stride) when not
+ * NULL.  No page may be a source and a destination, or a destination twice. */
+int hb_pages_copy(const hb_page_pool *pool, int n, const int32_t *src_dev, const int32_t *dst_dev,
+                  void *dst_pages_dev, int dst_n_pages, void *stream);
+
 /* Library-level error text (for calls that have no engine, e.g. hb_gemv). */
 const char *hb_library_error(void);
 
