@@ -5,7 +5,7 @@
 
 #include "hb_engine_impl.h"
 #include "hb_paged_ops.cuh"
-#include "hb_paged_rows.cuh"
+#include "hb_paged_tiles.cuh"
 
 using namespace hbi;
 namespace pg = hb::paged;
@@ -23,8 +23,11 @@ DeviceInfo g_devices[kMaxDevices];
 
 template <int D, class T>
 cudaError_t opt_in() {
-  return cudaFuncSetAttribute(pg::paged_rows_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              pg::RowsSize<D>::kSmem);
+  const cudaError_t err = cudaFuncSetAttribute(pg::paged_rows_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               pg::RowsSize<D>::kSmem);
+  if (err != cudaSuccess) return err;
+  return cudaFuncSetAttribute(pg::paged_tiles_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              pg::TilesSize<D>::kSmem);
 }
 
 // The current device's multiprocessors; the first call on a device also opts
@@ -58,7 +61,7 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Byte offsets of the workspace's regions.
 struct Regions {
-  size_t mark, need, off, fresh, from, to, held, stage, arrived, parts, total;
+  size_t mark, need, off, fresh, from, to, held, stage, arrived, arrived2, parts, parts2, total;
 };
 Regions regions(const hb_page_pool &p) {
   Regions r{};
@@ -72,6 +75,7 @@ Regions regions(const hb_page_pool &p) {
   };
   r.mark = take(slots * 4);
   r.arrived = take(2 * kMaxSms * 4);
+  r.arrived2 = take(2 * kMaxSms * 4);
   r.need = take(slots * 4);
   r.off = take(slots * 4);
   r.fresh = take(pages * 4);
@@ -81,6 +85,8 @@ Regions regions(const hb_page_pool &p) {
   r.stage = take(slots * static_cast<size_t>(p.table_width) * 4);
   const size_t rows = p.head_dim == 64 ? pg::RowsSize<64>::kPartFloats : pg::RowsSize<128>::kPartFloats;
   r.parts = take(static_cast<size_t>(rows_pieces(p.head_dim, kMaxSms)) * 2 * rows * 4);
+  const size_t tiles = p.head_dim == 64 ? pg::TilesSize<64>::kPartFloats : pg::TilesSize<128>::kPartFloats;
+  r.parts2 = take(static_cast<size_t>(kMaxSms) * 2 * 2 * tiles * 4);
   r.total = at;
   return r;
 }
@@ -171,9 +177,30 @@ int launch_copy(const hb_page_pool &p, void *to_pages, int to_n, const int *from
   return HB_OK;
 }
 
+// Which kernels an attention call launches: the rows kernel for entries of up
+// to 16 packed rows, the tiles kernel for the others, one of them where the
+// bound on an entry's rows (or, all being equal, their sum) says that it has
+// nothing to leave to the other.  A bound that is wrong costs time, not rows:
+// a kernel launched alone takes every entry.
 template <int D, class T>
-cudaError_t launch_rows(const pg::Attend &A, int grid, int least, cudaStream_t st) {
-  pg::paged_rows_kernel<D, T><<<grid, pg::kRowsThreads, pg::RowsSize<D>::kSmem, st>>>(A, least);
+cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) {
+  const pg::Batch &b = A.batch;
+  const int64_t most = static_cast<int64_t>(max_rows) * A.shape.group;
+  const bool rows_only = most <= pg::kRowsTile;
+  const bool tiles_only = !rows_only && static_cast<int64_t>(b.entries) * max_rows == b.rows;
+  A.few = rows_only ? INT32_MAX : tiles_only ? 0 : pg::kRowsTile;
+  if (!tiles_only) {
+    A.shape.tile = pg::kRowsTile;
+    A.shape.block = pg::kPage;
+    pg::paged_rows_kernel<D, T><<<rows_pieces(D, sms), pg::kRowsThreads, pg::RowsSize<D>::kSmem, st>>>(A, 2);
+  }
+  if (!rows_only) {
+    A.shape.tile = pg::kTilesTile;
+    A.shape.block = pg::kTilesBlock;
+    A.arrived = A.arrived2;
+    A.parts = A.parts2;
+    pg::paged_tiles_kernel<D, T><<<sms, pg::kTilesThreads, pg::TilesSize<D>::kSmem, st>>>(A, 4);
+  }
   return cudaGetLastError();
 }
 
@@ -206,7 +233,7 @@ int hb_paged_status(const hb_page_pool *pool, int32_t *status, void *stream) {
     HB_CUDA(nullptr, cudaMemsetAsync(pool->workspace_dev, 0, sizeof(c), st));
     if (c.ctrl.err) {   // a call that gave up may have left tiles half joined
       const Regions r = regions(*pool);
-      HB_CUDA(nullptr, cudaMemsetAsync(static_cast<uint8_t *>(pool->workspace_dev) + r.arrived, 0, 2 * kMaxSms * 4, st));
+      HB_CUDA(nullptr, cudaMemsetAsync(static_cast<uint8_t *>(pool->workspace_dev) + r.arrived, 0, r.need - r.arrived, st));
     }
     HB_CUDA(nullptr, cudaStreamSynchronize(st));
   }
@@ -258,15 +285,16 @@ int hb_paged_attend(const hb_page_pool *pool, int layer, const hb_paged_rows *ro
   A.arrived = reinterpret_cast<int *>(static_cast<uint8_t *>(pool->workspace_dev) + r.arrived);
   A.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(pool->workspace_dev) + r.parts);
   A.limit_ns = kDefaultLimitNs;
-  A.shape = pg::Shape{q->q_heads / pool->kv_heads, pool->table_width, q->window, pg::kRowsTile, pg::kPage};
+  A.arrived2 = reinterpret_cast<int *>(static_cast<uint8_t *>(pool->workspace_dev) + r.arrived2);
+  A.parts2 = reinterpret_cast<float *>(static_cast<uint8_t *>(pool->workspace_dev) + r.parts2);
+  A.shape = pg::Shape{q->q_heads / pool->kv_heads, pool->table_width, q->window, 0, 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int grid = rows_pieces(pool->head_dim, sms);
   const bool bf = pool->element == HB_ELEM_BF16;
-  const int least = 2;
+  const int most = rows->max_rows;
   if (pool->head_dim == 64)
-    HB_CUDA(nullptr, bf ? (launch_rows<64, __nv_bfloat16>(A, grid, least, st)) : (launch_rows<64, __half>(A, grid, least, st)));
+    HB_CUDA(nullptr, bf ? (launch_attend<64, __nv_bfloat16>(A, most, sms, st)) : (launch_attend<64, __half>(A, most, sms, st)));
   else
-    HB_CUDA(nullptr, bf ? (launch_rows<128, __nv_bfloat16>(A, grid, least, st)) : (launch_rows<128, __half>(A, grid, least, st)));
+    HB_CUDA(nullptr, bf ? (launch_attend<128, __nv_bfloat16>(A, most, sms, st)) : (launch_attend<128, __half>(A, most, sms, st)));
   return HB_OK;
 }
 

@@ -226,6 +226,32 @@ struct Elem<__half> {
   }
 };
 
+// 8 elements; VEC: the address is 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const uint16_t *p) {
+  if constexpr (VEC) {
+    return __ldg(reinterpret_cast<const uint4 *>(p));
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = static_cast<uint32_t>(p[2 * k]) | static_cast<uint32_t>(p[2 * k + 1]) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(uint16_t *p, const uint4 &v) {
+  if constexpr (VEC) {
+    *reinterpret_cast<uint4 *>(p) = v;
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      p[2 * k] = static_cast<uint16_t>(w[k]);
+      p[2 * k + 1] = static_cast<uint16_t>(w[k] >> 16);
+    }
+  }
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -246,8 +272,11 @@ struct Attend {
   Shape shape;
   float scale, scale_log2;         // of the scores; times log2(e)
   int q_vec, o_vec;                // q rows / out rows are 16-byte aligned
+  int few;                         // entries of up to this many packed rows are the rows kernel's, others the tiles'
   float *parts;                    // joined tiles: per piece two parts
   int *arrived;                    // per piece, zero between launches
+  float *parts2;                   // the tiles kernel's
+  int *arrived2;
   uint64_t limit_ns;
 };
 

@@ -55,29 +55,6 @@ __device__ __forceinline__ void rope8(const uint4 &x0, const uint4 &x1, const fl
   hi = make_uint4(h[0], h[1], h[2], h[3]);
 }
 
-// 8 elements; VEC: the address is 16-byte aligned.
-template <bool VEC>
-__device__ __forceinline__ uint4 load8(const uint16_t *p) {
-  if constexpr (VEC) return __ldg(reinterpret_cast<const uint4 *>(p));
-  uint32_t w[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) w[k] = static_cast<uint32_t>(p[2 * k]) | static_cast<uint32_t>(p[2 * k + 1]) << 16;
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <bool VEC>
-__device__ __forceinline__ void store8(uint16_t *p, const uint4 &v) {
-  if constexpr (VEC) {
-    *reinterpret_cast<uint4 *>(p) = v;
-  } else {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      p[2 * k] = static_cast<uint16_t>(w[k]);
-      p[2 * k + 1] = static_cast<uint16_t>(w[k] >> 16);
-    }
-  }
-}
-
 template <int D, class T, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ Append A) {
   __shared__ int s_pos[kAppendRows], s_page[kAppendRows];

@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
     fence_mbar_init();
   }
   if (threadIdx.x < kRowsTile) s_bad[threadIdx.x] = 0;
-  fill_prefix(A.pool, A.batch, S, s_prefix, [](const Entry &) { return true; });
+  fill_prefix(A.pool, A.batch, S, s_prefix, [&](const Entry &e) { return e.n * S.group <= A.few; });
   const int64_t total = s_prefix[A.batch.entries];
   const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + least - 1) / least));
   if (static_cast<int>(blockIdx.x) >= pieces) return;

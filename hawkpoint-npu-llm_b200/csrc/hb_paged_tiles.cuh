@@ -1,0 +1,559 @@
+// hb_paged_tiles.cuh -- attention over a paged cache for chunks and prompts, on
+// the 5th-generation tensor cores.
+//
+// o_i = sum_j softmax_j(scale q_i . k_j) v_j.  A tile is 256 packed rows (the q
+// heads of a kv head's group times consecutive rows), as two halves of 128,
+// the M of tcgen05.mma; a step is a block of 128 positions, two pages.  Per
+// half and step: S = Q K^T (128 x 128 x D) into TMEM; one thread a row reads
+// its 128 scores, keeps the running maximum and sum in FP32, and writes the
+// weights exp2(c s - c m) back to TMEM as 16-bit; O += P V with P from TMEM.
+// A page's K and V are operand tiles as they lie in the pool (128-byte
+// swizzled rows; V is the MN-major B), fetched by plain bulk copies.
+//
+// What bounds it: with heads of 64 a step's 2 x 2.1 MFLOP take the tensor
+// pipe 512 cycles a half, its 16,384 exponentials the 16-a-cycle special
+// function units 1,024: the softmax is the bound, and the two halves take
+// turns so that one's MMAs run under the other's exponentials.  With heads of
+// 128 both take 1,024 cycles.  O is rescaled only when a row's maximum has
+// grown by more than 2^8 (the sum and O share the stale maximum, so the
+// result is the same), which after the first blocks is almost never.
+//
+// Warps 0-3 and 4-7: the softmax of either half; warp 8: MMA issue; warp 9:
+// loads (10 and 11 only make up the warpgroup that gives registers to the
+// softmax).  One block a multiprocessor; the line of blocks is cut evenly
+// (hb_paged.cuh), a tile cut by a border is joined by the last of its pieces
+// to finish.
+#pragma once
+
+#include "hb_paged_rows.cuh"
+
+namespace hb {
+namespace paged {
+
+constexpr int kTilesTile = 256, kTilesHalf = 128, kTilesBlock = 128;
+constexpr int kTilesThreads = 384;
+// Registers a thread after the split: 256 softmax threads x 216 + 128 others x
+// 72 = 384 x 168, what the block is launched with.
+constexpr int kTilesRegs = 216, kOtherRegs = 72;
+
+template <int D>
+struct TilesSize {
+  static constexpr bool kEarly = D == 64;   // TMEM has room for P beside S: the next S starts before this P V
+  static constexpr int kOperand = (D / 64) * 16384;              // 128 rows or positions
+  static constexpr int kStages = D == 64 ? 8 : 4;
+  static constexpr int kSmem = 2 * kOperand + kStages * kOperand + 1024;
+  static constexpr uint32_t kS = 0, kO = 256, kP = D == 64 ? 384 : 0;   // TMEM columns; P of half h: + h * (64 or 128)
+  static constexpr uint32_t kPHalf = D == 64 ? 64 : 128;
+  static constexpr int kPartFloats = kTilesHalf * (D + 2);
+};
+
+// ---- PTX -------------------------------------------------------------------------------
+__device__ __forceinline__ void t_alloc(uint32_t *dst, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void t_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void t_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void t_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void t_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem], and A[tmem] B[smem]
+__device__ __forceinline__ void t_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void t_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// 32 consecutive 32-bit columns of this thread's TMEM lane.
+__device__ __forceinline__ void t_ld32(uint32_t taddr, float *r) {
+  uint32_t *u = reinterpret_cast<uint32_t *>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void t_st32(uint32_t taddr, const uint32_t *u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]),
+        "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]),
+        "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]),
+        "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+      : "memory");
+}
+__device__ __forceinline__ void t_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void t_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A 128-byte-swizzled shared-memory operand (rows of 128 bytes, groups of
+// eight rows 1 KB apart); `lead`: bytes between the 64-column parts of an
+// MN-major operand (a K-major one is addressed part by part).
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t saddr, uint32_t lead) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lead >> 4) & 0x3FFFu) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16, FP32 accumulator, M = 128, N = n; `mn`: B is MN-major.
+template <class T>
+__host__ __device__ constexpr uint32_t tiles_idesc(int n, bool mn) {
+  return (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+}
+
+// Barrier over a half's four softmax warps (barriers 2 and 3), ORing a predicate.
+__device__ __forceinline__ bool half_any(int half, bool pred) {
+  uint32_t out;
+  asm volatile(
+      "{\n\t.reg .pred p, r;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred r, %2, 128, p;\n\tselp.u32 %0, 1, 0, r;\n\t}"
+      : "=r"(out) : "r"(pred ? 1u : 0u), "r"(2 + half) : "memory");
+  return out != 0;
+}
+
+// mbar_wait without a call: the softmax threads wait with a row of scores in
+// registers, which a call would move to memory.
+__device__ __forceinline__ bool t_wait(uint64_t *bar, uint32_t parity, Ctrl *ctrl, uint64_t limit_ns, int where) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t start = globaltimer_ns();
+  while (!mbar_try_wait_suspend(bar, parity, 20000u)) {
+    if (ld_volatile_int(&ctrl->abort)) return false;
+    if (globaltimer_ns() - start > limit_ns) {
+      if (atomicCAS(&ctrl->err, 0, kErrTimeout) == 0) atomicExch(&ctrl->err_where, where);
+      atomicExch(&ctrl->abort, 1);
+      return false;
+    }
+  }
+  return true;
+}
+
+struct TilesBars {
+  uint64_t full[8], empty[8];                              // the ring of K and V blocks
+  uint64_t q_full[2], s_full[2], s_read[2], p_full[2], o_done[2];
+  uint64_t done;
+};
+
+template <int D, class T>
+__global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __grid_constant__ Attend A, int least) {
+  using E = Elem<T>;
+  using Z = TilesSize<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int64_t s_prefix[kMaxEntries + 1];
+  __shared__ TilesBars bars;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_last[2];
+  uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t *ring = smem + 2 * Z::kOperand;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Shape S = A.shape;
+  Ctrl *ctrl = &A.pool.control->ctrl;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Z::kStages; ++i) {
+      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.empty[i], 1);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&bars.q_full[h], 4);
+      mbar_init(&bars.s_full[h], 1);
+      mbar_init(&bars.s_read[h], 4);
+      mbar_init(&bars.p_full[h], 4);
+      mbar_init(&bars.o_done[h], 1);
+    }
+    mbar_init(&bars.done, 1);
+    fence_mbar_init();
+  }
+  fill_prefix(A.pool, A.batch, S, s_prefix, [&](const Entry &e) { return e.n * S.group > A.few; });
+  const int64_t total = s_prefix[A.batch.entries];
+  const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + least - 1) / least));
+  if (static_cast<int>(blockIdx.x) >= pieces) return;
+  if (warp == 0) t_alloc(&s_tmem, 512);
+  t_before();
+  __syncthreads();
+  t_after();
+  const uint32_t tmem = s_tmem;
+
+  Walk w;
+  w.u = piece_begin(total, pieces, blockIdx.x);
+  w.end = piece_begin(total, pieces, blockIdx.x + 1);
+  bool more = w.start(A.pool, A.batch, S, s_prefix);
+  auto halves = [&]() { return w.e.n * S.group - w.t * kTilesTile > kTilesHalf ? 2 : 1; };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp == 9) {
+    // ---- loads: K(0), then K(j + 1), V(j), the order the MMAs use them in
+    int it = 0;
+    bool ok = true;
+    auto load = [&](bool is_v, int block, int pg0, int pg1) {
+      const int s = it % Z::kStages;
+      const uint32_t ph = static_cast<uint32_t>(it / Z::kStages) & 1u;
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[s], ph ^ 1u, ctrl, A.limit_ns, kWhereEmpty)) != 0;
+      if (!ok) return;
+      uint8_t *dst = ring + s * Z::kOperand;
+      int held[2];
+      uint32_t bytes = 0;
+      bool wrote = false;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        held[x] = (x ? pg1 : pg0) < 0 ? 0 : max(0, min(kPage, w.e.length - (2 * block + x) * kPage));
+        bytes += (D / 64) * held[x] * 128;
+        if (is_v && held[x] < kPage) {   // V where there is no position: zero, so that weight zero times it is zero
+          for (int h = 0; h < D / 64; ++h)
+            for (int y = held[x] * 128 + lane * 16; y < kBlockBytes; y += 512)
+              *reinterpret_cast<uint4 *>(dst + h * 16384 + x * kBlockBytes + y) = make_uint4(0, 0, 0, 0);
+          wrote = true;
+        }
+      }
+      if (wrote) {
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) {
+        if (bytes) mbar_arrive_expect_tx(&bars.full[s], bytes); else mbar_arrive_count(&bars.full[s], 1);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (!held[x]) continue;
+          const uint8_t *src = kv_block(A, x ? pg1 : pg0, w.head) + (is_v ? D / 64 * kBlockBytes : 0);
+          for (int h = 0; h < D / 64; ++h)
+            bulk_g2s(dst + h * 16384 + x * kBlockBytes, src + h * kBlockBytes, held[x] * 128, &bars.full[s]);
+        }
+      }
+      __syncwarp();
+      ++it;
+    };
+    for (; more && ok; more = w.next(A.pool, A.batch, S, s_prefix)) {
+      const int first = w.first(), count = w.count();
+      int mine = -1, v0 = -1, v1 = -1;
+      for (int j = 0; j < count && ok; ++j) {
+        if ((j & 15) == 0) mine = page_of(A.pool, w.e.slot, 2 * (first + j) + lane);
+        const int k0 = __shfl_sync(0xffffffffu, mine, 2 * (j & 15)), k1 = __shfl_sync(0xffffffffu, mine, 2 * (j & 15) + 1);
+        load(false, first + j, k0, k1);
+        if (j > 0 && ok) load(true, first + j - 1, v0, v1);
+        v0 = k0;
+        v1 = k1;
+      }
+      if (ok) load(true, first + count - 1, v0, v1);
+    }
+    for (int i = max(0, it - Z::kStages); i < it; ++i)   // nothing in flight when the block ends
+      mbar_wait_quiet(&bars.full[i % Z::kStages], static_cast<uint32_t>(i / Z::kStages) & 1u, A.limit_ns);
+  } else if (warp == 8) {
+    // ---- MMA issue, one thread
+    if (lane == 0) {
+      constexpr uint32_t kIdescS = tiles_idesc<T>(kTilesBlock, false), kIdescO = tiles_idesc<T>(D, true);
+      int it = 0;                       // ring stages consumed
+      uint32_t n_q[2] = {0, 0}, n_s[2] = {0, 0};   // tiles and steps of either half so far
+      bool ok = true;
+      const uint32_t q_s = smem_u32(smem), r_s = smem_u32(ring);
+      auto wait = [&](uint64_t *bar, uint32_t phase) { ok = ok && mbar_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull); };
+      auto stage = [&](int i) { return i % Z::kStages; };
+      auto wait_ring = [&](int i) { wait(&bars.full[stage(i)], static_cast<uint32_t>(i / Z::kStages)); };
+      auto mma_s = [&](int h, int i) {   // S of half h from the K in ring use i
+        const uint32_t a = q_s + h * Z::kOperand, b = r_s + stage(i) * Z::kOperand;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+          t_mma_ss(tmem + Z::kS + h * 128, swizzled_desc(a + off, 16), swizzled_desc(b + off, 16), kIdescS, k != 0);
+        }
+        t_commit(&bars.s_full[h]);
+      };
+      auto mma_o = [&](int h, int i, bool fresh) {   // O of half h from the V in ring use i
+        const uint32_t b = r_s + stage(i) * Z::kOperand;
+#pragma unroll
+        for (int k = 0; k < kTilesBlock / 16; ++k)
+          t_mma_ts(tmem + Z::kO + h * D, tmem + Z::kP + h * Z::kPHalf + k * 8, swizzled_desc(b + k * 2048, 16384), kIdescO,
+                   !(fresh && k == 0));
+        t_commit(&bars.o_done[h]);
+      };
+      for (; more && ok; more = w.next(A.pool, A.batch, S, s_prefix)) {
+        const int count = w.count(), nh = halves();
+        for (int h = 0; h < nh; ++h) wait(&bars.q_full[h], n_q[h]++);
+        wait_ring(it);
+        if (!ok) break;
+        t_after();
+        for (int h = 0; h < nh; ++h) mma_s(h, it);
+        t_commit(&bars.empty[stage(it)]);
+        for (int j = 0; j < count && ok; ++j) {
+          const bool next = j + 1 < count;
+          const int ik = it + 2 * j + 1, iv = next ? ik + 1 : ik;
+          if (next) wait_ring(ik);
+          if constexpr (Z::kEarly) {
+            if (next) {
+              for (int h = 0; h < nh; ++h) {
+                wait(&bars.s_read[h], n_s[h]);
+                if (!ok) break;
+                t_after();
+                mma_s(h, ik);
+              }
+              t_commit(&bars.empty[stage(ik)]);
+            }
+            wait_ring(iv);
+            for (int h = 0; h < nh && ok; ++h) {
+              wait(&bars.p_full[h], n_s[h]++);
+              if (!ok) break;
+              t_after();
+              mma_o(h, iv, j == 0);
+            }
+            t_commit(&bars.empty[stage(iv)]);
+          } else {
+            wait_ring(iv);
+            for (int h = 0; h < nh && ok; ++h) {
+              wait(&bars.p_full[h], n_s[h]++);
+              if (!ok) break;
+              t_after();
+              mma_o(h, iv, j == 0);
+              if (next) mma_s(h, ik);   // over the P just used: MMAs run in order
+            }
+            if (next) t_commit(&bars.empty[stage(ik)]);
+            t_commit(&bars.empty[stage(iv)]);
+          }
+        }
+        it += 2 * count;
+      }
+      t_commit(&bars.done);   // after a give-up too: nothing in flight when TMEM is freed
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTilesRegs));
+    // ---- softmax of half h, a thread a row
+    const int h = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + Z::kS + h * 128 + lanes, t_o = tmem + Z::kO + h * D + lanes,
+                   t_p = tmem + Z::kP + h * Z::kPHalf + lanes;
+    const float c = A.scale_log2;
+    uint32_t steps = 0;   // of this half so far
+    bool ok = true;
+    auto wait = [&](uint64_t *bar, uint32_t phase) {
+      ok = __all_sync(0xffffffffu, ok && t_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
+      return ok;
+    };
+    for (; more; more = w.next(A.pool, A.batch, S, s_prefix)) {
+      if (h >= halves()) continue;
+      const int packed = w.e.n * S.group, row = w.t * kTilesTile + h * kTilesHalf + r;
+      const int first = w.first(), count = w.count();
+      const bool in = row < packed;
+      const int i = row / S.group, g = row - i * S.group;
+      const int pos = in ? w.e.length - w.e.n + i : -1;
+      {
+        // this row's q into the operand tile
+        const T *q = static_cast<const T *>(A.q) + (in ? (w.e.row0 + i) * A.q_row + (w.head * S.group + g) * A.q_head : 0);
+        uint8_t *dst = smem + h * Z::kOperand + r * 128;
+        uint4 v[D / 8];
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+          v[x] = make_uint4(0, 0, 0, 0);
+          if (in) v[x] = A.q_vec ? __ldg(reinterpret_cast<const uint4 *>(q) + x) : load8<false>(reinterpret_cast<const uint16_t *>(q) + 8 * x);
+        }
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x)
+          *reinterpret_cast<uint4 *>(dst + (x >> 3) * 16384 + (((x & 7) ^ (r & 7)) << 4)) = v[x];
+        fence_proxy_async_smem();
+        t_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_count(&bars.q_full[h], 1);
+      }
+      // whether every page of the piece's blocks is there
+      bool hole = false;
+      for (int x = r; x < 2 * count; x += 128) {
+        const int p = 2 * first + x;
+        hole |= p * kPage < w.e.length && page_of(A.pool, w.e.slot, p) < 0;
+      }
+      hole = half_any(h, hole);
+      // positions that every row of the half sees need no mask
+      const int lead = (w.t * kTilesTile + h * kTilesHalf) / S.group;
+      const int tail = (min(packed, w.t * kTilesTile + (h + 1) * kTilesHalf) - 1) / S.group;
+      const int all_hi = w.e.length - w.e.n + lead;
+      const int all_lo = S.window > 0 ? w.e.length - w.e.n + tail - S.window + 1 : 0;
+
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < count; ++j, ++steps) {
+        if (!wait(&bars.s_full[h], steps)) break;
+        t_after();
+        float s[128];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) t_ld32(t_s + x * 32, s + x * 32);
+        t_ld_wait();
+        if constexpr (Z::kEarly) {
+          t_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_count(&bars.s_read[h], 1);
+        }
+        const int j0 = (first + j) * kTilesBlock;
+        if (hole || j0 + kTilesBlock - 1 > all_hi || j0 < all_lo) {
+          const int hi = pos - j0, lo = S.window > 0 ? hi - S.window : -1;   // sees lo < x <= hi
+          const bool p0 = !hole || page_of(A.pool, w.e.slot, 2 * (first + j)) >= 0;
+          const bool p1 = !hole || page_of(A.pool, w.e.slot, 2 * (first + j) + 1) >= 0;
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (x > hi || x <= lo || !(x < 64 ? p0 : p1)) s[x] = -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int x = 4; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {   // also from m = -inf; both -inf: NaN, no
+          const float nm = fmaxf(m, top), a = nm == -INFINITY ? 1.f : exp2_approx((m - nm) * c);
+          m = nm;
+          l *= a;
+          if (j > 0) {
+            if (!wait(&bars.o_done[h], steps - 1)) break;
+            t_after();
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+              float o[32];
+              t_ld32(t_o + x * 32, o);
+              t_ld_wait();
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] *= a;
+              t_st32(t_o + x * 32, reinterpret_cast<const uint32_t *>(o));
+            }
+          }
+        }
+        if constexpr (Z::kEarly) {   // P is free when the last step's P V has read it
+          if (j > 0 && !wait(&bars.o_done[h], steps - 1)) break;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t p[32];
+#pragma unroll
+          for (int y = 0; y < 32; ++y) {
+            const float a = exp2_approx(fmaf(s[x * 64 + 2 * y], c, -mc));
+            const float b = exp2_approx(fmaf(s[x * 64 + 2 * y + 1], c, -mc));
+            sum[(2 * y) & 3] += a;
+            sum[(2 * y + 1) & 3] += b;
+            p[y] = E::pack(a, b);
+          }
+          t_st32(t_p + x * 32, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        t_st_wait();
+        t_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_count(&bars.p_full[h], 1);
+      }
+      if (ok) wait(&bars.o_done[h], steps - 1);
+      t_after();
+      const bool whole = w.u == w.tile_u && w.tile_u + w.units <= w.end;
+      constexpr int64_t kTwo = 2 * Z::kPartFloats;   // a part has two halves
+      if (half_any(h, !ok)) break;   // a wait gave up: the control block says which
+      bool write = in;
+      int c0 = 0, c1 = -1;
+      if (!whole) {
+        // a tile that other pieces share: leave this part, and the last of
+        // them to arrive joins all parts in order; [D / 4][128] of 4 floats
+        float *part = A.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (w.u == w.tile_u ? 1 : 0)) * kTwo + h * Z::kPartFloats;
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+          float o[32];
+          t_ld32(t_o + x * 32, o);
+          t_ld_wait();
+#pragma unroll
+          for (int y = 0; y < 8; ++y)
+            __stcg(reinterpret_cast<float4 *>(part) + (x * 8 + y) * 128 + r,
+                   make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]));
+        }
+        __stcg(part + 128 * D + r, m);
+        __stcg(part + 128 * (D + 1) + r, l);
+        __threadfence();
+        half_any(h, false);
+        c0 = piece_of(total, pieces, w.tile_u);
+        c1 = piece_of(total, pieces, w.tile_u + w.units - 1);
+        if (r == 0) {
+          const int before = atomicAdd(&A.arrived[2 * c0 + h], 1);
+          s_last[h] = before == c1 - c0;
+          if (s_last[h]) A.arrived[2 * c0 + h] = 0;
+        }
+        half_any(h, false);
+        write = write && s_last[h] != 0;
+        if (write) {
+          __threadfence();
+          const float *p = A.parts + h * Z::kPartFloats + 128 * D + r;
+          m = -INFINITY;
+          for (int k = c0; k <= c1; ++k) m = fmaxf(m, __ldcg(p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo));
+          l = 0.f;
+          for (int k = c0; k <= c1; ++k) {
+            const float *pk = p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo;
+            l = fmaf(__ldcg(pk + 128), exp2_approx((__ldcg(pk) - (m == -INFINITY ? 0.f : m)) * c), l);
+          }
+        }
+      }
+      bool bad = false;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T *out = static_cast<T *>(A.out) + (w.e.row0 + i) * A.o_row + (w.head * S.group + g) * A.o_head;
+#pragma unroll 1
+      for (int x = 0; x < D / 32; ++x) {
+        float o[32];
+        if (whole) {
+          t_ld32(t_o + x * 32, o);
+          t_ld_wait();
+        } else if (write) {
+          const float *p = A.parts + h * Z::kPartFloats;
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[y] = 0.f;
+          for (int k = c0; k <= c1; ++k) {
+            const float *pk = p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo;
+            const float f = exp2_approx((__ldcg(pk + 128 * D + r) - (m == -INFINITY ? 0.f : m)) * c);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const float4 v = __ldcg(reinterpret_cast<const float4 *>(pk) + (x * 8 + y) * 128 + r);
+              o[4 * y] = fmaf(v.x, f, o[4 * y]);
+              o[4 * y + 1] = fmaf(v.y, f, o[4 * y + 1]);
+              o[4 * y + 2] = fmaf(v.z, f, o[4 * y + 2]);
+              o[4 * y + 3] = fmaf(v.w, f, o[4 * y + 3]);
+            }
+          }
+        }
+        if (write) {
+#pragma unroll
+          for (int y = 0; y < 32; ++y) {
+            o[y] = l == 0.f ? 0.f : o[y] * inv;
+            bad |= !(fabsf(o[y]) <= 3.4e38f);
+          }
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint4 v = make_uint4(E::pack(o[8 * y], o[8 * y + 1]), E::pack(o[8 * y + 2], o[8 * y + 3]),
+                                       E::pack(o[8 * y + 4], o[8 * y + 5]), E::pack(o[8 * y + 6], o[8 * y + 7]));
+            uint16_t *dst = reinterpret_cast<uint16_t *>(out) + x * 32 + y * 8;
+            if (A.o_vec) store8<true>(dst, v); else store8<false>(dst, v);
+          }
+        }
+      }
+      if (write && A.lse != nullptr)
+        A.lse[static_cast<int64_t>(w.e.row0 + i) * A.q_heads + w.head * S.group + g] =
+            l == 0.f ? -INFINITY : m * A.scale + logf(l);
+      t_before();   // this half's O and S are read: its next q and p arrivals say so
+      // rows with infinities or NaN: each again, alone, by its own warp
+      unsigned again = __ballot_sync(0xffffffffu, bad);
+      while (again) {
+        const int x = __ffs(again) - 1;
+        again &= again - 1;
+        const int y = w.t * kTilesTile + h * kTilesHalf + (warp & 3) * 32 + x;
+        __syncwarp();
+        row_alone<D, T>(A, w.e, w.head, y / S.group, y % S.group);
+      }
+      half_any(h, false);   // s_last may be written again
+    }
+  }
+  __syncwarp();
+  // every MMA has completed before TMEM is freed
+  mbar_wait_quiet(&bars.done, 0, A.limit_ns);
+  t_before();
+  __syncthreads();
+  t_after();
+  if (warp == 0) t_dealloc(tmem, 512);
+}
+
+}  // namespace paged
+}  // namespace hb

@@ -3,8 +3,8 @@ against plain implementations: attention in float64, append bit for bit, the
 page operators against books kept in Python.
 
 Attention tolerance, per element of a row with weights w_j (float64) over the
-positions it sees: the output is rounded once (u |o|, u = 2^-9 for BF16, 2^-12
-for FP16), the weights once (u A, A = sum w_j |v_j|; FP16 weights below its
+positions it sees: the output is rounded once (u |o|, u = 2^-8 for BF16's 8
+significant bits, 2^-11 for FP16's 11), the weights once (u A, A = sum w_j |v_j|; FP16 weights below its
 normal range by 2^-25 each, on a scale that lets the largest weight be as
 small as 2^-8), and FP32 scores are off by at most (head_dim + 8) 2^-24 S, S
 the largest sum |q||k| scale, which moves a weight by twice that, relatively;
@@ -93,7 +93,7 @@ class Case:
         """(out, lse, tolerance of out, tolerance of lse) in float64, position by position of the table."""
         torch = _torch()
         scale = self.d ** -0.5 if scale is None else scale
-        u = 2.0 ** -9 if self.dtype == torch.bfloat16 else 2.0 ** -12
+        u = 2.0 ** -8 if self.dtype == torch.bfloat16 else 2.0 ** -11
         pool, group = self.cache.pool, self.qh // self.kvh
         table = self.cache.table.cpu().numpy()
         out = torch.zeros((self.n_rows, self.qh, self.d), dtype=torch.float64, device="cuda")
@@ -125,7 +125,7 @@ class Case:
                     a = w @ torch.nan_to_num(vis, nan=0.0, posinf=0.0, neginf=0.0).abs()
                     big = torch.where(hide, 0.0, (q.abs() @ k.abs().T * scale)).amax(1, keepdim=True)
                     ds = (self.d + 8) * 2.0 ** -24 * torch.nan_to_num(big, nan=0.0, posinf=0.0)
-                    tail = len(seen) * 2.0 ** -17 if u < 2.0 ** -10 else 0.0
+                    tail = len(seen) * 2.0 ** -17 if u < 2.0 ** -9 else 0.0
                     out[at: at + n, h] = o
                     lse[at: at + n, h] = torch.logsumexp(s, 1)
                     tol[at: at + n, h] = u * o.abs() + (u + 2 * ds + 2.0 ** -18) * a + 2.0 ** -8 * u * tail + 2.0 ** -24
