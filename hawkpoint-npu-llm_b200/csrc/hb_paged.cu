@@ -24,10 +24,10 @@ DeviceInfo g_devices[kMaxDevices];
 template <int D, class T>
 cudaError_t opt_in() {
   const cudaError_t err = cudaFuncSetAttribute(pg::paged_rows_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               pg::RowsSize<D>::kSmem);
+                                               static_cast<int>(pg::RowsSize<D>::kSmem + pg::line_bytes(pg::kMaxEntries)));
   if (err != cudaSuccess) return err;
   return cudaFuncSetAttribute(pg::paged_tiles_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              pg::TilesSize<D>::kSmem);
+                              static_cast<int>(pg::TilesSize<D>::kSmem + pg::line_bytes(pg::kMaxEntries)));
 }
 
 // The current device's multiprocessors; the first call on a device also opts
@@ -188,18 +188,19 @@ cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) 
   const int64_t most = static_cast<int64_t>(max_rows) * A.shape.group;
   const bool rows_only = most <= pg::kRowsTile;
   const bool tiles_only = !rows_only && static_cast<int64_t>(b.entries) * max_rows == b.rows;
+  const size_t line = pg::line_bytes(b.entries);
   A.few = rows_only ? INT32_MAX : tiles_only ? 0 : pg::kRowsTile;
   if (!tiles_only) {
     A.shape.tile = pg::kRowsTile;
     A.shape.block = pg::kPage;
-    pg::paged_rows_kernel<D, T><<<rows_pieces(D, sms), pg::kRowsThreads, pg::RowsSize<D>::kSmem, st>>>(A, 2);
+    pg::paged_rows_kernel<D, T><<<rows_pieces(D, sms), pg::kRowsThreads, pg::RowsSize<D>::kSmem + line, st>>>(A, 2);
   }
   if (!rows_only) {
     A.shape.tile = pg::kTilesTile;
     A.shape.block = pg::kTilesBlock;
     A.arrived = A.arrived2;
     A.parts = A.parts2;
-    pg::paged_tiles_kernel<D, T><<<sms, pg::kTilesThreads, pg::TilesSize<D>::kSmem, st>>>(A, 4);
+    pg::paged_tiles_kernel<D, T><<<sms, pg::kTilesThreads, pg::TilesSize<D>::kSmem + line, st>>>(A, 4);
   }
   return cudaGetLastError();
 }

@@ -94,37 +94,60 @@ __device__ __forceinline__ int tile_units(const Shape &S, const Entry &e, int t)
 }
 __device__ __forceinline__ int tiles_of(const Shape &S, const Entry &e) { return (e.n * S.group + S.tile - 1) / S.tile; }
 
-// The line of a call: prefix[b] = units before entry b (shared memory,
-// kMaxEntries + 1), filled by all threads of the block.  `take(entry)` says
-// whether this kernel takes an entry's rows.
+// The line of a call: its entries and prefix[b], the units before entry b, in
+// shared memory.
+struct Line {
+  int64_t *prefix;   // [entries + 1]
+  Entry *entry;      // [entries]
+};
+__host__ __device__ inline size_t line_bytes(int entries) {
+  return (static_cast<size_t>(entries) * (8 + sizeof(Entry)) + 8 + 15) / 16 * 16;
+}
+__device__ __forceinline__ Line line_at(uint8_t *smem, int entries) {
+  return Line{reinterpret_cast<int64_t *>(smem + entries * sizeof(Entry)), reinterpret_cast<Entry *>(smem)};
+}
+
+// Fills the line, by all threads of the block: a thread an entry, so that the
+// entries' reads are in flight together; the tiles of a long entry are
+// counted by its warp.  `take(entry)`: whether this kernel takes its rows.
 template <class Take>
-__device__ __forceinline__ void fill_prefix(const Pool &P, const Batch &B, const Shape &S, int64_t *prefix,
-                                            const Take &take) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  for (int b = warp; b < B.entries; b += warps) {
-    const Entry e = entry_of(P, B, b);
+__device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const Shape &S, const Line &line,
+                                          const Take &take) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int b0 = warp * 32; b0 < B.entries; b0 += blockDim.x) {
+    const int b = b0 + lane;
+    Entry e{0, 0, 0, -1};
+    if (b < B.entries) line.entry[b] = e = entry_of(P, B, b);
+    const int tiles = b < B.entries && take(e) ? tiles_of(S, e) : 0;
     int64_t u = 0;
-    if (take(e))
-      for (int t = lane; t < tiles_of(S, e); t += 32) u += tile_units(S, e, t);
+    if (tiles <= 4)
+      for (int t = 0; t < tiles; ++t) u += tile_units(S, e, t);
+    for (unsigned many = __ballot_sync(0xffffffffu, tiles > 4); many; many &= many - 1) {
+      const int x = __ffs(many) - 1, n = __shfl_sync(0xffffffffu, tiles, x);
+      const Entry y{0, __shfl_sync(0xffffffffu, e.n, x), __shfl_sync(0xffffffffu, e.length, x), 0};
+      int v = 0;
+      for (int t = lane; t < n; t += 32) v += tile_units(S, y, t);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-    if (lane == 0) prefix[b + 1] = u * P.kv_heads;
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == x) u = v;
+    }
+    if (b < B.entries) line.prefix[b + 1] = u * P.kv_heads;
   }
   __syncthreads();
   if (warp == 0) {
     int64_t base = 0;
     for (int b0 = 0; b0 < B.entries; b0 += 32) {
       const int b = b0 + lane;
-      int64_t v = b < B.entries ? prefix[b + 1] : 0;
+      int64_t v = b < B.entries ? line.prefix[b + 1] : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += w;
       }
-      if (b < B.entries) prefix[b + 1] = base + v;
+      if (b < B.entries) line.prefix[b + 1] = base + v;
       base += __shfl_sync(0xffffffffu, v, 31);
     }
-    if (lane == 0) prefix[0] = 0;
+    if (lane == 0) line.prefix[0] = 0;
   }
   __syncthreads();
 }
@@ -138,15 +161,16 @@ struct Walk {
   Span span;
 
   // positions on the tile that holds unit u; false when the piece is done
-  __device__ __forceinline__ bool start(const Pool &P, const Batch &B, const Shape &S, const int64_t *prefix) {
+  __device__ __forceinline__ bool start(const Pool &P, const Batch &B, const Shape &S, const Line &line) {
     if (u >= end) return false;
+    const int64_t *prefix = line.prefix;
     int lo = 0, hi = B.entries - 1;
-    while (lo < hi) {  // the last entry whose prefix is <= u and that has units
+    while (lo < hi) {  // the entry that holds unit u
       const int mid = (lo + hi) >> 1;
       if (prefix[mid + 1] > u) hi = mid; else lo = mid + 1;
     }
     b = lo;
-    e = entry_of(P, B, b);
+    e = line.entry[b];
     const int64_t per = (prefix[b + 1] - prefix[b]) / P.kv_heads;
     const int64_t rem = u - prefix[b];
     head = static_cast<int>(rem / per);
@@ -165,7 +189,7 @@ struct Walk {
   __device__ __forceinline__ int count() const {
     return static_cast<int>(min(end, tile_u + units) - u);
   }
-  __device__ __forceinline__ bool next(const Pool &P, const Batch &B, const Shape &S, const int64_t *prefix) {
+  __device__ __forceinline__ bool next(const Pool &P, const Batch &B, const Shape &S, const Line &line) {
     u = tile_u + units;
     if (u >= end) return false;
     if (t + 1 < tiles_of(S, e)) {
@@ -182,7 +206,7 @@ struct Walk {
       span = tile_span(S, e, 0);
       return true;
     }
-    return start(P, B, S, prefix);
+    return start(P, B, S, line);
   }
 };
 

@@ -114,13 +114,13 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
   using E = Elem<T>;
   using Z = RowsSize<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ int64_t s_prefix[kMaxEntries + 1];
   __shared__ __align__(8) uint64_t s_full[Z::kStages], s_empty[Z::kStages];
   __shared__ int s_valid[Z::kStages];
   __shared__ float s_m[kRowsWarps][kRowsTile], s_l[kRowsWarps][kRowsTile];
   __shared__ int s_bad[kRowsTile], s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Shape S = A.shape;
+  const Line line = line_at(smem + Z::kSmem, A.batch.entries);
   Ctrl *ctrl = &A.pool.control->ctrl;
 
   if (threadIdx.x == 0) {
@@ -131,19 +131,19 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
     fence_mbar_init();
   }
   if (threadIdx.x < kRowsTile) s_bad[threadIdx.x] = 0;
-  fill_prefix(A.pool, A.batch, S, s_prefix, [&](const Entry &e) { return e.n * S.group <= A.few; });
-  const int64_t total = s_prefix[A.batch.entries];
+  fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group <= A.few; });
+  const int64_t total = line.prefix[A.batch.entries];
   const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + least - 1) / least));
   if (static_cast<int>(blockIdx.x) >= pieces) return;
   Walk w;
   w.u = piece_begin(total, pieces, blockIdx.x);
   w.end = piece_begin(total, pieces, blockIdx.x + 1);
-  bool more = w.start(A.pool, A.batch, S, s_prefix);
+  bool more = w.start(A.pool, A.batch, S, line);
   int it = 0;  // stages used so far
 
   if (warp == kRowsWarps) {
     bool ok = true;
-    for (; more && ok; more = w.next(A.pool, A.batch, S, s_prefix)) {
+    for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
       const int first = w.first(), count = w.count();
       for (int k0 = 0; k0 < count && ok; k0 += 32) {
         const int mine = k0 + lane < count ? page_of(A.pool, w.e.slot, first + k0 + lane) : -1;
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
   float *join = reinterpret_cast<float *>(smem + Z::kStages * Z::kStageBytes);
   const int mat = lane >> 3, mrow = lane & 7;
   bool ok = true;
-  for (; more; more = w.next(A.pool, A.batch, S, s_prefix)) {
+  for (; more; more = w.next(A.pool, A.batch, S, line)) {
     const int packed = w.e.n * S.group;
     // this thread's rows of the tile: r, r + 8
     const int r0 = w.t * kRowsTile + (lane >> 2);

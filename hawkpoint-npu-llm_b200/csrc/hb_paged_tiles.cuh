@@ -99,11 +99,15 @@ __device__ __forceinline__ void t_ld_wait() { asm volatile("tcgen05.wait::ld.syn
 __device__ __forceinline__ void t_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // A 128-byte-swizzled shared-memory operand (rows of 128 bytes, groups of
-// eight rows 1 KB apart); `lead`: bytes between the 64-column parts of an
-// MN-major operand (a K-major one is addressed part by part).
-__device__ __forceinline__ uint64_t swizzled_desc(uint32_t saddr, uint32_t lead) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lead >> 4) & 0x3FFFu) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// eight rows 1 KB apart) as the low word of its descriptor, to which 16-byte
+// steps are added; `lead`: bytes between the 64-column parts of an MN-major
+// operand (a K-major one is addressed part by part).
+__device__ __forceinline__ uint32_t swizzled_lo(uint32_t saddr, uint32_t lead) {
+  return (saddr >> 4) | ((lead >> 4) << 16);
+}
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t lo) {
+  constexpr uint32_t kHi = (1024 >> 4) | (1u << 14) | (2u << 29);   // 8-row step, version, 128-byte swizzle
+  return static_cast<uint64_t>(kHi) << 32 | lo;
 }
 // kind::f16, FP32 accumulator, M = 128, N = n; `mn`: B is MN-major.
 template <class T>
@@ -148,7 +152,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   using E = Elem<T>;
   using Z = TilesSize<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int64_t s_prefix[kMaxEntries + 1];
   __shared__ TilesBars bars;
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
@@ -156,6 +159,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   uint8_t *ring = smem + 2 * Z::kOperand;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Shape S = A.shape;
+  const Line line = line_at(smem + (2 + Z::kStages) * Z::kOperand, A.batch.entries);
   Ctrl *ctrl = &A.pool.control->ctrl;
 
   if (threadIdx.x == 0) {
@@ -173,8 +177,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     mbar_init(&bars.done, 1);
     fence_mbar_init();
   }
-  fill_prefix(A.pool, A.batch, S, s_prefix, [&](const Entry &e) { return e.n * S.group > A.few; });
-  const int64_t total = s_prefix[A.batch.entries];
+  fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group > A.few; });
+  const int64_t total = line.prefix[A.batch.entries];
   const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + least - 1) / least));
   if (static_cast<int>(blockIdx.x) >= pieces) return;
   if (warp == 0) t_alloc(&s_tmem, 512);
@@ -186,7 +190,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   Walk w;
   w.u = piece_begin(total, pieces, blockIdx.x);
   w.end = piece_begin(total, pieces, blockIdx.x + 1);
-  bool more = w.start(A.pool, A.batch, S, s_prefix);
+  bool more = w.start(A.pool, A.batch, S, line);
   auto halves = [&]() { return w.e.n * S.group - w.t * kTilesTile > kTilesHalf ? 2 : 1; };
 
   if (warp >= 8) {
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       __syncwarp();
       ++it;
     };
-    for (; more && ok; more = w.next(A.pool, A.batch, S, s_prefix)) {
+    for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
       const int first = w.first(), count = w.count();
       int mine = -1, v0 = -1, v1 = -1;
       for (int j = 0; j < count && ok; ++j) {
@@ -254,28 +258,30 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       int it = 0;                       // ring stages consumed
       uint32_t n_q[2] = {0, 0}, n_s[2] = {0, 0};   // tiles and steps of either half so far
       bool ok = true;
-      const uint32_t q_s = smem_u32(smem), r_s = smem_u32(ring);
+      constexpr uint32_t kStep = Z::kOperand >> 4;
+      const uint32_t q_lo = swizzled_lo(smem_u32(smem), 16), k_lo = swizzled_lo(smem_u32(ring), 16),
+                     v_lo = swizzled_lo(smem_u32(ring), 16384);
       auto wait = [&](uint64_t *bar, uint32_t phase) { ok = ok && mbar_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull); };
       auto stage = [&](int i) { return i % Z::kStages; };
       auto wait_ring = [&](int i) { wait(&bars.full[stage(i)], static_cast<uint32_t>(i / Z::kStages)); };
       auto mma_s = [&](int h, int i) {   // S of half h from the K in ring use i
-        const uint32_t a = q_s + h * Z::kOperand, b = r_s + stage(i) * Z::kOperand;
+        const uint32_t a = q_lo + h * kStep, b = k_lo + stage(i) * kStep;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          t_mma_ss(tmem + Z::kS + h * 128, swizzled_desc(a + off, 16), swizzled_desc(b + off, 16), kIdescS, k != 0);
+          const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+          t_mma_ss(tmem + Z::kS + h * 128, swizzled_desc(a + off), swizzled_desc(b + off), kIdescS, k != 0);
         }
         t_commit(&bars.s_full[h]);
       };
       auto mma_o = [&](int h, int i, bool fresh) {   // O of half h from the V in ring use i
-        const uint32_t b = r_s + stage(i) * Z::kOperand;
+        const uint32_t b = v_lo + stage(i) * kStep;
 #pragma unroll
         for (int k = 0; k < kTilesBlock / 16; ++k)
-          t_mma_ts(tmem + Z::kO + h * D, tmem + Z::kP + h * Z::kPHalf + k * 8, swizzled_desc(b + k * 2048, 16384), kIdescO,
+          t_mma_ts(tmem + Z::kO + h * D, tmem + Z::kP + h * Z::kPHalf + k * 8, swizzled_desc(b + k * (2048 >> 4)), kIdescO,
                    !(fresh && k == 0));
         t_commit(&bars.o_done[h]);
       };
-      for (; more && ok; more = w.next(A.pool, A.batch, S, s_prefix)) {
+      for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
         const int count = w.count(), nh = halves();
         for (int h = 0; h < nh; ++h) wait(&bars.q_full[h], n_q[h]++);
         wait_ring(it);
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       ok = __all_sync(0xffffffffu, ok && t_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
       return ok;
     };
-    for (; more; more = w.next(A.pool, A.batch, S, s_prefix)) {
+    for (; more; more = w.next(A.pool, A.batch, S, line)) {
       if (h >= halves()) continue;
       const int packed = w.e.n * S.group, row = w.t * kTilesTile + h * kTilesHalf + r;
       const int first = w.first(), count = w.count();
