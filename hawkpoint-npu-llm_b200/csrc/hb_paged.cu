@@ -193,11 +193,13 @@ cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) 
   if (!tiles_only) {
     A.shape.tile = pg::kRowsTile;
     A.shape.block = pg::kPage;
+    A.shape.extra = pg::kRowsExtra;
     pg::paged_rows_kernel<D, T><<<rows_pieces(D, sms), pg::kRowsThreads, pg::RowsSize<D>::kSmem + line, st>>>(A, 2);
   }
   if (!rows_only) {
     A.shape.tile = pg::kTilesTile;
     A.shape.block = pg::kTilesBlock;
+    A.shape.extra = pg::kTilesExtra;
     A.arrived = A.arrived2;
     A.parts = A.parts2;
     pg::paged_tiles_kernel<D, T><<<sms, pg::kTilesThreads, pg::TilesSize<D>::kSmem + line, st>>>(A, 4);
@@ -288,7 +290,10 @@ int hb_paged_attend(const hb_page_pool *pool, int layer, const hb_paged_rows *ro
   A.limit_ns = kDefaultLimitNs;
   A.arrived2 = reinterpret_cast<int *>(static_cast<uint8_t *>(pool->workspace_dev) + r.arrived2);
   A.parts2 = reinterpret_cast<float *>(static_cast<uint8_t *>(pool->workspace_dev) + r.parts2);
-  A.shape = pg::Shape{q->q_heads / pool->kv_heads, pool->table_width, q->window, 0, 0};
+  A.shape.group = q->q_heads / pool->kv_heads;
+  A.shape.width = pool->table_width;
+  A.shape.window = q->window;
+  A.shape.group_inv = static_cast<uint32_t>(0xFFFFFFFFull / static_cast<uint32_t>(A.shape.group));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = pool->element == HB_ELEM_BF16;
   const int most = rows->max_rows;

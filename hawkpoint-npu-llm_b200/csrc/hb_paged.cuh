@@ -67,12 +67,18 @@ __device__ __forceinline__ Entry entry_of(const Pool &P, const Batch &B, int b) 
 // The rows of an entry and the q heads of a kv head's group are packed into
 // tiles of `tile` rows: packed row r is row r / group, head r % group.  A
 // tile's work is the blocks of `block` positions that any of its rows sees
-// (one at least, so that a tile without any is still written).  The blocks of
-// all tiles, entry by entry, head by head, are one line that the thread
-// blocks cut into equal pieces, so ragged lengths leave none idle; a tile cut
-// by a border is joined from its parts.
+// (one at least, so that a tile without any is still written), and `extra`
+// units for its start and end.  The units of all tiles, entry by entry, head
+// by head, are one line that the thread blocks cut into equal pieces, so ragged
+// lengths leave none idle; a tile cut by a border is joined from its parts.
 struct Shape {
-  int group, width, window, tile, block;
+  int group, width, window, tile, block, extra;
+  uint32_t group_inv;   // 2^32 / group, rounded down (at most 2^32 - 1)
+  // r / group for r >= 0: the product is at most one too low
+  __device__ __forceinline__ int row_of(int r) const {
+    const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(r), group_inv));
+    return r - q * group >= group ? q + 1 : q;
+  }
 };
 
 struct Span {
@@ -81,16 +87,18 @@ struct Span {
 
 __device__ __forceinline__ Span tile_span(const Shape &S, const Entry &e, int t) {
   const int packed = e.n * S.group;
-  const int i0 = t * S.tile / S.group, i1 = (min(packed, (t + 1) * S.tile) - 1) / S.group;
+  const int i0 = S.row_of(t * S.tile), i1 = S.row_of(min(packed, (t + 1) * S.tile) - 1);
   const int last = e.length - e.n + i1, first = e.length - e.n + i0;
+  // blocks are 64 or 128 positions: shifts
+  const int shift = S.block == 128 ? 7 : 6;
   Span s;
-  s.hi = last < 0 ? 0 : min(last / S.block, (S.width * kPage - 1) / S.block) + 1;
-  s.lo = S.window > 0 ? max(0, first - S.window + 1) / S.block : 0;
+  s.hi = last < 0 ? 0 : min(last >> shift, (S.width * kPage - 1) >> shift) + 1;
+  s.lo = S.window > 0 ? max(0, first - S.window + 1) >> shift : 0;
   return s;
 }
 __device__ __forceinline__ int tile_units(const Shape &S, const Entry &e, int t) {
   const Span s = tile_span(S, e, t);
-  return max(1, s.hi - s.lo);
+  return max(1, s.hi - s.lo) + S.extra;
 }
 __device__ __forceinline__ int tiles_of(const Shape &S, const Entry &e) { return (e.n * S.group + S.tile - 1) / S.tile; }
 
@@ -152,15 +160,23 @@ __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const S
   __syncthreads();
 }
 
-// A walk over the tiles of one piece [u, end) of the line.
+// A walk over the tiles of one piece [u, end) of the line, the same in every
+// lane of the warps that make it.
 struct Walk {
   int64_t u, end;        // units left
-  int64_t tile_u;        // first unit of the current tile
-  int b, head, t, units;
+  int64_t tile_u;        // first unit of the current tile, its extra ones included
+  int b, head, t, units, tiles, blocks_before;
   Entry e;
   Span span;
 
-  // positions on the tile that holds unit u; false when the piece is done
+  __device__ __forceinline__ void at(const Shape &S, int tile) {
+    t = tile;
+    span = tile_span(S, e, t);
+    units = max(1, span.hi - span.lo) + S.extra;
+    // where the piece enters the tile's blocks
+    blocks_before = static_cast<int>(max(static_cast<int64_t>(0), u - tile_u - S.extra));
+  }
+  // On the tile that holds unit u; false when the piece is done.
   __device__ __forceinline__ bool start(const Pool &P, const Batch &B, const Shape &S, const Line &line) {
     if (u >= end) return false;
     const int64_t *prefix = line.prefix;
@@ -171,42 +187,68 @@ struct Walk {
     }
     b = lo;
     e = line.entry[b];
-    const int64_t per = (prefix[b + 1] - prefix[b]) / P.kv_heads;
-    const int64_t rem = u - prefix[b];
-    head = static_cast<int>(rem / per);
-    tile_u = prefix[b] + head * per;
-    t = 0;
-    units = tile_units(S, e, 0);
-    while (tile_u + units <= u) {
-      tile_u += units;
-      units = tile_units(S, e, ++t);
+    tiles = tiles_of(S, e);
+    int64_t rem = u - prefix[b];
+    head = 0;
+    if (P.kv_heads > 1) {
+      const int64_t per = (prefix[b + 1] - prefix[b]) / P.kv_heads;
+      head = static_cast<int>(rem / per);
+      rem -= head * per;
     }
-    span = tile_span(S, e, t);
-    return true;
+    tile_u = u - rem;
+    int tile = 0;
+    const int lane = threadIdx.x & 31;
+    for (int t0 = 0; tiles > 1; t0 += 32) {   // a lane a tile: the one that holds the unit
+      const int mine = t0 + lane < tiles ? tile_units(S, e, t0 + lane) : 0;
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, sum > rem);
+      if (past) {
+        const int x = __ffs(past) - 1;
+        tile = t0 + x;
+        tile_u += __shfl_sync(0xffffffffu, sum - mine, x);
+        break;
+      }
+      const int all = __shfl_sync(0xffffffffu, sum, 31);
+      rem -= all;
+      tile_u += all;
+    }
+    at(S, tile);
+    return end > tile_u + S.extra;   // else the piece ends before the tile's first block
   }
-  // blocks of the tile that lie in the piece: [first, first + count)
-  __device__ __forceinline__ int first() const { return span.lo + static_cast<int>(u - tile_u); }
-  __device__ __forceinline__ int count() const {
-    return static_cast<int>(min(end, tile_u + units) - u);
+  // the piece's blocks of the tile: [first, first + count)
+  __device__ __forceinline__ int first() const { return span.lo + blocks_before; }
+  __device__ __forceinline__ int count(const Shape &S) const {
+    return static_cast<int>(min(end, tile_u + units) - tile_u) - S.extra - blocks_before;
   }
+  __device__ __forceinline__ bool opens() const { return blocks_before == 0; }
+  __device__ __forceinline__ bool whole() const { return opens() && tile_u + units <= end; }
   __device__ __forceinline__ bool next(const Pool &P, const Batch &B, const Shape &S, const Line &line) {
     u = tile_u + units;
-    if (u >= end) return false;
-    if (t + 1 < tiles_of(S, e)) {
+    if (u + S.extra >= end) return false;
+    if (t + 1 < tiles) {
       tile_u = u;
-      units = tile_units(S, e, ++t);
-      span = tile_span(S, e, t);
+      at(S, t + 1);
       return true;
     }
     if (head + 1 < P.kv_heads) {
       ++head;
-      t = 0;
       tile_u = u;
-      units = tile_units(S, e, 0);
-      span = tile_span(S, e, 0);
+      at(S, 0);
       return true;
     }
-    return start(P, B, S, line);
+    // the next entry that has units
+    do ++b; while (line.prefix[b + 1] == u);
+    e = line.entry[b];
+    tiles = tiles_of(S, e);
+    head = 0;
+    tile_u = u;
+    at(S, 0);
+    return true;
   }
 };
 

@@ -20,6 +20,7 @@ namespace hb {
 namespace paged {
 
 constexpr int kRowsTile = 16;
+constexpr int kRowsExtra = 1;                       // a tile's start and end, in pages
 constexpr int kRowsWarps = 4;                       // consumer warps
 constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
 template <int D>
@@ -84,7 +85,7 @@ template <int D, class T, int kPer>
 __device__ __forceinline__ bool store_row(const Attend &A, const Entry &e, int head, int r, int d0, const float *o,
                                           float m, float l) {
   using E = Elem<T>;
-  const int i = r / A.shape.group, g = r - i * A.shape.group;
+  const int i = A.shape.row_of(r), g = r - i * A.shape.group;
   const int64_t row = e.row0 + i;
   const int qh = head * A.shape.group + g;
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
   if (warp == kRowsWarps) {
     bool ok = true;
     for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
-      const int first = w.first(), count = w.count();
+      const int first = w.first(), count = w.count(S);
       for (int k0 = 0; k0 < count && ok; k0 += 32) {
         const int mine = k0 + lane < count ? page_of(A.pool, w.e.slot, first + k0 + lane) : -1;
         for (int k = k0; k < min(count, k0 + 32); ++k, ++it) {
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
     const T *qrow[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = r0 + 8 * h, i = r / S.group, g = r - i * S.group;
+      const int r = r0 + 8 * h, i = S.row_of(r), g = r - i * S.group;
       const bool in = r < packed;
       pos[h] = in ? w.e.length - w.e.n + i : -1;
       qrow[h] = static_cast<const T *>(A.q) +
@@ -213,8 +214,8 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
         qa[ks][x] = q_pair<T>(A, qrow[x & 1], ks * 16 + (x >> 1) * 8 + (lane & 3) * 2, r0 + 8 * (x & 1) < packed);
     // positions that every row of the tile sees need no mask
     const int tail = min(packed, (w.t + 1) * kRowsTile) - 1;
-    const int all_hi = w.e.length - w.e.n + w.t * kRowsTile / S.group;
-    const int all_lo = S.window > 0 ? w.e.length - w.e.n + tail / S.group - S.window + 1 : 0;
+    const int all_hi = w.e.length - w.e.n + S.row_of(w.t * kRowsTile);
+    const int all_lo = S.window > 0 ? w.e.length - w.e.n + S.row_of(tail) - S.window + 1 : 0;
 
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float o[D / 8][4];
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[n][x] = 0.f;
 
-    const int first = w.first(), count = w.count();
+    const int first = w.first(), count = w.count(S);
     for (int k = 0; k < count; ++k, ++it) {
       const int s = it % Z::kStages;
       const uint32_t ph = static_cast<uint32_t>(it / Z::kStages) & 1u;
@@ -328,12 +329,12 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
       }
     }
     const int row = w.t * kRowsTile + r;
-    const bool whole = w.u == w.tile_u && w.tile_u + w.units <= w.end;
+    const bool whole = w.whole();
     bool write = row < packed;
     if (!whole) {
       // a tile that other pieces share: leave this part, and the last of
       // them to arrive joins all parts in order
-      float *part = A.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (w.u == w.tile_u ? 1 : 0)) * Z::kPartFloats;
+      float *part = A.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (w.opens() ? 1 : 0)) * Z::kPartFloats;
       if (write) {
 #pragma unroll
         for (int d = 0; d < kPer; d += 4)
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
       }
       __threadfence();
       rows_sync();
-      const int c0 = piece_of(total, pieces, w.tile_u);
+      const int c0 = piece_of(total, pieces, w.tile_u + S.extra);
       const int c1 = piece_of(total, pieces, w.tile_u + w.units - 1);
       if (threadIdx.x == 0) {
         const int before = atomicAdd(&A.arrived[c0], 1);

@@ -19,8 +19,7 @@
 // result is the same), which after the first blocks is almost never.
 //
 // Warps 0-3 and 4-7: the softmax of either half; warp 8: MMA issue; warp 9:
-// loads (10 and 11 only make up the warpgroup that gives registers to the
-// softmax).  One block a multiprocessor; the line of blocks is cut evenly
+// K and V; warps 10 and 11: the halves' q, a tile ahead.  One block a multiprocessor; the line of blocks is cut evenly
 // (hb_paged.cuh), a tile cut by a border is joined by the last of its pieces
 // to finish.
 #pragma once
@@ -31,6 +30,7 @@ namespace hb {
 namespace paged {
 
 constexpr int kTilesTile = 256, kTilesHalf = 128, kTilesBlock = 128;
+constexpr int kTilesExtra = 2;   // a tile's start and end, in blocks
 constexpr int kTilesThreads = 384;
 // Registers a thread after the split: 256 softmax threads x 216 + 128 others x
 // 72 = 384 x 168, what the block is launched with.
@@ -143,7 +143,7 @@ __device__ __forceinline__ bool t_wait(uint64_t *bar, uint32_t parity, Ctrl *ctr
 
 struct TilesBars {
   uint64_t full[8], empty[8];                              // the ring of K and V blocks
-  uint64_t q_full[2], s_full[2], s_read[2], p_full[2], o_done[2];
+  uint64_t q_full[2], q_empty[2], s_full[2], s_read[2], p_full[2], o_done[2];
   uint64_t done;
 };
 
@@ -168,7 +168,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       mbar_init(&bars.empty[i], 1);
     }
     for (int h = 0; h < 2; ++h) {
-      mbar_init(&bars.q_full[h], 4);
+      mbar_init(&bars.q_full[h], 1);
+      mbar_init(&bars.q_empty[h], 1);
       mbar_init(&bars.s_full[h], 1);
       mbar_init(&bars.s_read[h], 4);
       mbar_init(&bars.p_full[h], 4);
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       ++it;
     };
     for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
-      const int first = w.first(), count = w.count();
+      const int first = w.first(), count = w.count(S);
       int mine = -1, v0 = -1, v1 = -1;
       for (int j = 0; j < count && ok; ++j) {
         if ((j & 15) == 0) mine = page_of(A.pool, w.e.slot, 2 * (first + j) + lane);
@@ -252,81 +253,119 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     for (int i = max(0, it - Z::kStages); i < it; ++i)   // nothing in flight when the block ends
       mbar_wait_quiet(&bars.full[i % Z::kStages], static_cast<uint32_t>(i / Z::kStages) & 1u, A.limit_ns);
   } else if (warp == 8) {
-    // ---- MMA issue, one thread
-    if (lane == 0) {
-      constexpr uint32_t kIdescS = tiles_idesc<T>(kTilesBlock, false), kIdescO = tiles_idesc<T>(D, true);
-      int it = 0;                       // ring stages consumed
-      uint32_t n_q[2] = {0, 0}, n_s[2] = {0, 0};   // tiles and steps of either half so far
-      bool ok = true;
-      constexpr uint32_t kStep = Z::kOperand >> 4;
-      const uint32_t q_lo = swizzled_lo(smem_u32(smem), 16), k_lo = swizzled_lo(smem_u32(ring), 16),
-                     v_lo = swizzled_lo(smem_u32(ring), 16384);
-      auto wait = [&](uint64_t *bar, uint32_t phase) { ok = ok && mbar_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull); };
-      auto stage = [&](int i) { return i % Z::kStages; };
-      auto wait_ring = [&](int i) { wait(&bars.full[stage(i)], static_cast<uint32_t>(i / Z::kStages)); };
-      auto mma_s = [&](int h, int i) {   // S of half h from the K in ring use i
-        const uint32_t a = q_lo + h * kStep, b = k_lo + stage(i) * kStep;
+    // ---- MMA issue: the warp walks, its first lane issues
+    constexpr uint32_t kIdescS = tiles_idesc<T>(kTilesBlock, false), kIdescO = tiles_idesc<T>(D, true);
+    int it = 0;                                  // ring stages consumed
+    uint32_t n_q[2] = {0, 0}, n_s[2] = {0, 0};   // tiles and steps of either half so far
+    bool ok = true;
+    constexpr uint32_t kStep = Z::kOperand >> 4;
+    const uint32_t q_lo = swizzled_lo(smem_u32(smem), 16), k_lo = swizzled_lo(smem_u32(ring), 16),
+                   v_lo = swizzled_lo(smem_u32(ring), 16384);
+    auto wait = [&](uint64_t *bar, uint32_t phase) {
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
+      return ok;
+    };
+    auto stage = [&](int i) { return i % Z::kStages; };
+    auto wait_ring = [&](int i) { return wait(&bars.full[stage(i)], static_cast<uint32_t>(i / Z::kStages)); };
+    auto commit = [&](uint64_t *bar) {
+      if (lane == 0) t_commit(bar);
+    };
+    auto mma_s = [&](int h, int i) {   // S of half h from the K in ring use i
+      t_after();
+      const uint32_t a = q_lo + h * kStep, b = k_lo + stage(i) * kStep;
+      if (lane == 0) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
           t_mma_ss(tmem + Z::kS + h * 128, swizzled_desc(a + off), swizzled_desc(b + off), kIdescS, k != 0);
         }
         t_commit(&bars.s_full[h]);
-      };
-      auto mma_o = [&](int h, int i, bool fresh) {   // O of half h from the V in ring use i
-        const uint32_t b = v_lo + stage(i) * kStep;
+      }
+    };
+    auto mma_o = [&](int h, int i, bool fresh) {   // O of half h from the V in ring use i
+      t_after();
+      const uint32_t b = v_lo + stage(i) * kStep;
+      if (lane == 0) {
 #pragma unroll
         for (int k = 0; k < kTilesBlock / 16; ++k)
-          t_mma_ts(tmem + Z::kO + h * D, tmem + Z::kP + h * Z::kPHalf + k * 8, swizzled_desc(b + k * (2048 >> 4)), kIdescO,
-                   !(fresh && k == 0));
+          t_mma_ts(tmem + Z::kO + h * D, tmem + Z::kP + h * Z::kPHalf + k * 8, swizzled_desc(b + k * (2048 >> 4)),
+                   kIdescO, !(fresh && k == 0));
         t_commit(&bars.o_done[h]);
-      };
-      for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
-        const int count = w.count(), nh = halves();
-        for (int h = 0; h < nh; ++h) wait(&bars.q_full[h], n_q[h]++);
-        wait_ring(it);
-        if (!ok) break;
-        t_after();
-        for (int h = 0; h < nh; ++h) mma_s(h, it);
-        t_commit(&bars.empty[stage(it)]);
-        for (int j = 0; j < count && ok; ++j) {
-          const bool next = j + 1 < count;
-          const int ik = it + 2 * j + 1, iv = next ? ik + 1 : ik;
-          if (next) wait_ring(ik);
-          if constexpr (Z::kEarly) {
-            if (next) {
-              for (int h = 0; h < nh; ++h) {
-                wait(&bars.s_read[h], n_s[h]);
-                if (!ok) break;
-                t_after();
-                mma_s(h, ik);
-              }
-              t_commit(&bars.empty[stage(ik)]);
-            }
-            wait_ring(iv);
-            for (int h = 0; h < nh && ok; ++h) {
-              wait(&bars.p_full[h], n_s[h]++);
-              if (!ok) break;
-              t_after();
-              mma_o(h, iv, j == 0);
-            }
-            t_commit(&bars.empty[stage(iv)]);
-          } else {
-            wait_ring(iv);
-            for (int h = 0; h < nh && ok; ++h) {
-              wait(&bars.p_full[h], n_s[h]++);
-              if (!ok) break;
-              t_after();
+      }
+    };
+    for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
+      const int count = w.count(S), nh = halves();
+      // S is free: the last step's P of either half, which was waited for,
+      // was written after its S was read
+      for (int h = 0; h < nh; ++h) wait(&bars.q_full[h], n_q[h]++);
+      if (!wait_ring(it)) break;
+      for (int h = 0; h < nh; ++h) mma_s(h, it);
+      commit(&bars.empty[stage(it)]);
+      if (count == 1)
+        for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h]);
+      for (int j = 0; j < count && ok; ++j) {
+        const bool next = j + 1 < count;
+        const int ik = it + 2 * j + 1, iv = next ? ik + 1 : ik;
+        if (next && !wait_ring(ik)) break;
+        if constexpr (Z::kEarly) {
+          if (next) {
+            for (int h = 0; h < nh; ++h)
+              if (wait(&bars.s_read[h], n_s[h])) mma_s(h, ik);
+            commit(&bars.empty[stage(ik)]);
+            if (j + 2 == count)
+              for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h]);
+          }
+          if (!wait_ring(iv)) break;
+          for (int h = 0; h < nh; ++h)
+            if (wait(&bars.p_full[h], n_s[h]++)) mma_o(h, iv, j == 0);
+          commit(&bars.empty[stage(iv)]);
+        } else {
+          if (!wait_ring(iv)) break;
+          for (int h = 0; h < nh; ++h)
+            if (wait(&bars.p_full[h], n_s[h]++)) {
               mma_o(h, iv, j == 0);
               if (next) mma_s(h, ik);   // over the P just used: MMAs run in order
             }
-            if (next) t_commit(&bars.empty[stage(ik)]);
-            t_commit(&bars.empty[stage(iv)]);
-          }
+          if (next) commit(&bars.empty[stage(ik)]);
+          commit(&bars.empty[stage(iv)]);
+          if (j + 2 == count)
+            for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h]);
         }
-        it += 2 * count;
       }
-      t_commit(&bars.done);   // after a give-up too: nothing in flight when TMEM is freed
+      it += 2 * count;
+    }
+    commit(&bars.done);   // after a give-up too: nothing in flight when TMEM is freed
+  } else {
+    // ---- warps 10, 11: the q rows of half h, a tile ahead of its softmax
+    const int h = warp - 10;
+    uint32_t n = 0;
+    bool ok = true;
+    for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
+      if (h >= halves()) continue;
+      ok = __all_sync(0xffffffffu, n == 0 || mbar_wait(&bars.q_empty[h], (n - 1) & 1u, ctrl, A.limit_ns, kWhereEmpty)) != 0;
+      if (!ok) break;
+      ++n;
+      const int packed = w.e.n * S.group, base = w.t * kTilesTile + h * kTilesHalf;
+      uint8_t *dst = smem + h * Z::kOperand;
+      // a lane 16 bytes; D / 8 lanes a row
+      const int c = lane % (D / 8);
+      for (int r = lane / (D / 8); r < kTilesHalf; r += 256 / D) {
+        uint8_t *to = dst + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        const int row = base + r, i = S.row_of(row), g = row - i * S.group;
+        const uint16_t *q = static_cast<const uint16_t *>(A.q) + (w.e.row0 + i) * A.q_row +
+                            (w.head * S.group + g) * A.q_head + c * 8;
+        if (row >= packed)
+          *reinterpret_cast<uint4 *>(to) = make_uint4(0, 0, 0, 0);
+        else if (A.q_vec)
+          cp_async16(to, q);
+        else
+          *reinterpret_cast<uint4 *>(to) = load8<false>(q);
+      }
+      cp_async_commit();
+      cp_async_wait_all();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_count(&bars.q_full[h], 1);
     }
   }
   } else {
@@ -346,28 +385,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     for (; more; more = w.next(A.pool, A.batch, S, line)) {
       if (h >= halves()) continue;
       const int packed = w.e.n * S.group, row = w.t * kTilesTile + h * kTilesHalf + r;
-      const int first = w.first(), count = w.count();
+      const int first = w.first(), count = w.count(S);
       const bool in = row < packed;
-      const int i = row / S.group, g = row - i * S.group;
+      const int i = S.row_of(row), g = row - i * S.group;
       const int pos = in ? w.e.length - w.e.n + i : -1;
-      {
-        // this row's q into the operand tile
-        const T *q = static_cast<const T *>(A.q) + (in ? (w.e.row0 + i) * A.q_row + (w.head * S.group + g) * A.q_head : 0);
-        uint8_t *dst = smem + h * Z::kOperand + r * 128;
-        uint4 v[D / 8];
-#pragma unroll
-        for (int x = 0; x < D / 8; ++x) {
-          v[x] = make_uint4(0, 0, 0, 0);
-          if (in) v[x] = A.q_vec ? __ldg(reinterpret_cast<const uint4 *>(q) + x) : load8<false>(reinterpret_cast<const uint16_t *>(q) + 8 * x);
-        }
-#pragma unroll
-        for (int x = 0; x < D / 8; ++x)
-          *reinterpret_cast<uint4 *>(dst + (x >> 3) * 16384 + (((x & 7) ^ (r & 7)) << 4)) = v[x];
-        fence_proxy_async_smem();
-        t_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_count(&bars.q_full[h], 1);
-      }
       // whether every page of the piece's blocks is there
       bool hole = false;
       for (int x = r; x < 2 * count; x += 128) {
@@ -376,8 +397,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       }
       hole = half_any(h, hole);
       // positions that every row of the half sees need no mask
-      const int lead = (w.t * kTilesTile + h * kTilesHalf) / S.group;
-      const int tail = (min(packed, w.t * kTilesTile + (h + 1) * kTilesHalf) - 1) / S.group;
+      const int lead = S.row_of(w.t * kTilesTile + h * kTilesHalf);
+      const int tail = S.row_of(min(packed, w.t * kTilesTile + (h + 1) * kTilesHalf) - 1);
       const int all_hi = w.e.length - w.e.n + lead;
       const int all_lo = S.window > 0 ? w.e.length - w.e.n + tail - S.window + 1 : 0;
 
@@ -451,7 +472,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       }
       if (ok) wait(&bars.o_done[h], steps - 1);
       t_after();
-      const bool whole = w.u == w.tile_u && w.tile_u + w.units <= w.end;
+      const bool whole = w.whole();
       constexpr int64_t kTwo = 2 * Z::kPartFloats;   // a part has two halves
       if (half_any(h, !ok)) break;   // a wait gave up: the control block says which
       bool write = in;
@@ -459,7 +480,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       if (!whole) {
         // a tile that other pieces share: leave this part, and the last of
         // them to arrive joins all parts in order; [D / 4][128] of 4 floats
-        float *part = A.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (w.u == w.tile_u ? 1 : 0)) * kTwo + h * Z::kPartFloats;
+        float *part = A.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (w.opens() ? 1 : 0)) * kTwo + h * Z::kPartFloats;
 #pragma unroll
         for (int x = 0; x < D / 32; ++x) {
           float o[32];
@@ -474,7 +495,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         __stcg(part + 128 * (D + 1) + r, l);
         __threadfence();
         half_any(h, false);
-        c0 = piece_of(total, pieces, w.tile_u);
+        c0 = piece_of(total, pieces, w.tile_u + S.extra);
         c1 = piece_of(total, pieces, w.tile_u + w.units - 1);
         if (r == 0) {
           const int before = atomicAdd(&A.arrived[2 * c0 + h], 1);
@@ -539,7 +560,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       if (write && A.lse != nullptr)
         A.lse[static_cast<int64_t>(w.e.row0 + i) * A.q_heads + w.head * S.group + g] =
             l == 0.f ? -INFINITY : m * A.scale + logf(l);
-      t_before();   // this half's O and S are read: its next q and p arrivals say so
+      t_before();   // this half's O is read: its next p arrival says so
       // rows with infinities or NaN: each again, alone, by its own warp
       unsigned again = __ballot_sync(0xffffffffu, bad);
       while (again) {
