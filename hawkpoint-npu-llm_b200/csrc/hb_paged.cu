@@ -155,8 +155,9 @@ pg::Scratch scratch_view(const hb_page_pool &p, const Regions &r) {
   return pg::Scratch{at(r.mark), at(r.need), at(r.off), at(r.fresh), at(r.from), at(r.to), at(r.held), at(r.stage)};
 }
 
-bool vec_ok(const void *base, int64_t a, int64_t b) {
-  return ((reinterpret_cast<uintptr_t>(base) | static_cast<uintptr_t>(a * 2) | static_cast<uintptr_t>(b * 2)) & 15) == 0;
+// Rows at a base and with strides (elements) that all are multiples of `bytes`.
+bool vec_ok(const void *base, int64_t a, int64_t b, unsigned bytes = 16) {
+  return ((reinterpret_cast<uintptr_t>(base) | static_cast<uintptr_t>(a * 2) | static_cast<uintptr_t>(b * 2)) & (bytes - 1)) == 0;
 }
 
 // The copy kernel after a books kernel, launched early.
@@ -285,6 +286,7 @@ int hb_paged_attend(const hb_page_pool *pool, int layer, const hb_paged_rows *ro
   A.scale_log2 = q->scale * 1.4426950408889634f;
   A.q_vec = vec_ok(q->q_dev, q->q_row_stride, q->q_head_stride);
   A.o_vec = vec_ok(q->out_dev, q->out_row_stride, q->out_head_stride);
+  A.o_wide = vec_ok(q->out_dev, q->out_row_stride, q->out_head_stride, 32);
   A.arrived = reinterpret_cast<int *>(static_cast<uint8_t *>(pool->workspace_dev) + r.arrived);
   A.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(pool->workspace_dev) + r.parts);
   A.limit_ns = kDefaultLimitNs;

@@ -338,6 +338,7 @@ struct Attend {
   Shape shape;
   float scale, scale_log2;         // of the scores; times log2(e)
   int q_vec, o_vec;                // q rows / out rows are 16-byte aligned
+  int o_wide;                      // 32-byte aligned
   int few;                         // entries of up to this many packed rows are the rows kernel's, others the tiles'
   float *parts;                    // joined tiles: per piece two parts
   int *arrived;                    // per piece, zero between launches

@@ -41,7 +41,8 @@ struct TilesSize {
   static constexpr bool kEarly = D == 64;   // TMEM has room for P beside S: the next S starts before this P V
   static constexpr int kOperand = (D / 64) * 16384;              // 128 rows or positions
   static constexpr int kStages = D == 64 ? 8 : 4;
-  static constexpr int kSmem = 2 * kOperand + kStages * kOperand + 1024;
+  static constexpr int kQ = D == 64 ? 2 : 1;                     // q buffers of either half
+  static constexpr int kSmem = (2 * kQ + kStages) * kOperand + 1024;
   static constexpr uint32_t kS = 0, kO = 256, kP = D == 64 ? 384 : 0;   // TMEM columns; P of half h: + h * (64 or 128)
   static constexpr uint32_t kPHalf = D == 64 ? 64 : 128;
   static constexpr int kPartFloats = kTilesHalf * (D + 2);
@@ -98,6 +99,46 @@ __device__ __forceinline__ void t_st32(uint32_t taddr, const uint32_t *u) {
 __device__ __forceinline__ void t_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void t_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two FP32 operations an instruction.
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_split(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 32 bytes at a 32-byte-aligned address.
+__device__ __forceinline__ void store32(void *p, const uint32_t *u) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]),
+               "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]) : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // A 128-byte-swizzled shared-memory operand (rows of 128 bytes, groups of
 // eight rows 1 KB apart) as the low word of its descriptor, to which 16-byte
 // steps are added; `lead`: bytes between the 64-column parts of an MN-major
@@ -116,15 +157,6 @@ __host__ __device__ constexpr uint32_t tiles_idesc(int n, bool mn) {
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
 }
 
-// Barrier over a half's four softmax warps (barriers 2 and 3), ORing a predicate.
-__device__ __forceinline__ bool half_any(int half, bool pred) {
-  uint32_t out;
-  asm volatile(
-      "{\n\t.reg .pred p, r;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred r, %2, 128, p;\n\tselp.u32 %0, 1, 0, r;\n\t}"
-      : "=r"(out) : "r"(pred ? 1u : 0u), "r"(2 + half) : "memory");
-  return out != 0;
-}
-
 // mbar_wait without a call: the softmax threads wait with a row of scores in
 // registers, which a call would move to memory.
 __device__ __forceinline__ bool t_wait(uint64_t *bar, uint32_t parity, Ctrl *ctrl, uint64_t limit_ns, int where) {
@@ -141,9 +173,28 @@ __device__ __forceinline__ bool t_wait(uint64_t *bar, uint32_t parity, Ctrl *ctr
   return true;
 }
 
+// A tile as the q warps tell it to the MMA and softmax warps.
+struct TileInfo {
+  int count;             // blocks; 0: there are no more tiles
+  int first;             // first block
+  int base, packed;      // the half's first packed row; the entry's rows
+  int row0, n, length, slot, head;
+  int two;               // both halves have rows
+  int whole, opens;      // the piece has all its blocks; the first of them
+  int hole;              // a page of the blocks is missing
+  int c0, c1;            // not whole: the pieces that share it
+};
+// A slot is written again four tiles later, when the q buffers' barriers say
+// that the softmax is past its tile.
+constexpr int kInfoSlots = 4;
+
 struct TilesBars {
   uint64_t full[8], empty[8];                              // the ring of K and V blocks
-  uint64_t q_full[2], q_empty[2], s_full[2], s_read[2], p_full[2], o_done[2];
+  uint64_t q_full[2][2], q_empty[2][2];                    // [half][buffer]
+  uint64_t s_full[2], s_read[2], p_full[2], o_done[2];
+  uint64_t i_full[2][kInfoSlots];                          // a tile is told: what the softmax, which MMAs of
+                                                           // short tiles may run ahead of, waits for
+  uint64_t half[2];                                        // a half's four softmax warps
   uint64_t done;
 };
 
@@ -154,12 +205,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   extern __shared__ uint8_t smem_raw[];
   __shared__ TilesBars bars;
   __shared__ uint32_t s_tmem;
+  __shared__ TileInfo s_info[2][kInfoSlots];
   __shared__ int s_last[2];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t *ring = smem + 2 * Z::kOperand;
+  uint8_t *ring = smem + 2 * Z::kQ * Z::kOperand;   // behind the q of either half, kQ tiles
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Shape S = A.shape;
-  const Line line = line_at(smem + (2 + Z::kStages) * Z::kOperand, A.batch.entries);
+  const Line line = line_at(smem + (2 * Z::kQ + Z::kStages) * Z::kOperand, A.batch.entries);
   Ctrl *ctrl = &A.pool.control->ctrl;
 
   if (threadIdx.x == 0) {
@@ -168,12 +220,16 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       mbar_init(&bars.empty[i], 1);
     }
     for (int h = 0; h < 2; ++h) {
-      mbar_init(&bars.q_full[h], 1);
-      mbar_init(&bars.q_empty[h], 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&bars.q_full[h][x], 1);
+        mbar_init(&bars.q_empty[h][x], 1);
+      }
       mbar_init(&bars.s_full[h], 1);
       mbar_init(&bars.s_read[h], 4);
       mbar_init(&bars.p_full[h], 4);
       mbar_init(&bars.o_done[h], 1);
+      mbar_init(&bars.half[h], 4);
+      for (int x = 0; x < kInfoSlots; ++x) mbar_init(&bars.i_full[h][x], 1);
     }
     mbar_init(&bars.done, 1);
     fence_mbar_init();
@@ -272,7 +328,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     };
     auto mma_s = [&](int h, int i) {   // S of half h from the K in ring use i
       t_after();
-      const uint32_t a = q_lo + h * kStep, b = k_lo + stage(i) * kStep;
+      const uint32_t a = q_lo + ((n_q[h] - 1) % Z::kQ * 2 + h) * kStep, b = k_lo + stage(i) * kStep;
       if (lane == 0) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -293,16 +349,23 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         t_commit(&bars.o_done[h]);
       }
     };
-    for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
-      const int count = w.count(S), nh = halves();
+    while (ok) {
+      if (!wait(&bars.q_full[0][n_q[0] % Z::kQ], n_q[0] / Z::kQ)) break;
+      const TileInfo &info = s_info[0][n_q[0] % kInfoSlots];
+      const int count = info.count, nh = info.two ? 2 : 1;
+      if (count == 0) break;
       // S is free: the last step's P of either half, which was waited for,
       // was written after its S was read
-      for (int h = 0; h < nh; ++h) wait(&bars.q_full[h], n_q[h]++);
+      ++n_q[0];
+      if (nh == 2) {
+        wait(&bars.q_full[1][n_q[1] % Z::kQ], n_q[1] / Z::kQ);
+        ++n_q[1];
+      }
       if (!wait_ring(it)) break;
       for (int h = 0; h < nh; ++h) mma_s(h, it);
       commit(&bars.empty[stage(it)]);
       if (count == 1)
-        for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h]);
+        for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h][(n_q[h] - 1) % Z::kQ]);
       for (int j = 0; j < count && ok; ++j) {
         const bool next = j + 1 < count;
         const int ik = it + 2 * j + 1, iv = next ? ik + 1 : ik;
@@ -313,7 +376,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
               if (wait(&bars.s_read[h], n_s[h])) mma_s(h, ik);
             commit(&bars.empty[stage(ik)]);
             if (j + 2 == count)
-              for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h]);
+              for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h][(n_q[h] - 1) % Z::kQ]);
           }
           if (!wait_ring(iv)) break;
           for (int h = 0; h < nh; ++h)
@@ -329,7 +392,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
           if (next) commit(&bars.empty[stage(ik)]);
           commit(&bars.empty[stage(iv)]);
           if (j + 2 == count)
-            for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h]);
+            for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h][(n_q[h] - 1) % Z::kQ]);
         }
       }
       it += 2 * count;
@@ -340,13 +403,22 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     const int h = warp - 10;
     uint32_t n = 0;
     bool ok = true;
-    for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
-      if (h >= halves()) continue;
-      ok = __all_sync(0xffffffffu, n == 0 || mbar_wait(&bars.q_empty[h], (n - 1) & 1u, ctrl, A.limit_ns, kWhereEmpty)) != 0;
-      if (!ok) break;
-      ++n;
+    while (ok) {
+      while (more && h >= halves()) more = w.next(A.pool, A.batch, S, line);
+      const int buf = n % Z::kQ;
+      ok = __all_sync(0xffffffffu, n < Z::kQ || mbar_wait(&bars.q_empty[h][buf], (n / Z::kQ - 1) & 1u, ctrl, A.limit_ns,
+                                                          kWhereEmpty)) != 0;
+      TileInfo &info = s_info[h][n % kInfoSlots];
+      if (!more || !ok) {
+        if (lane == 0) {
+          info.count = 0;
+          mbar_arrive_count(&bars.q_full[h][buf], 1);
+          mbar_arrive_count(&bars.i_full[h][n % kInfoSlots], 1);
+        }
+        break;
+      }
       const int packed = w.e.n * S.group, base = w.t * kTilesTile + h * kTilesHalf;
-      uint8_t *dst = smem + h * Z::kOperand;
+      uint8_t *dst = smem + (buf * 2 + h) * Z::kOperand;
       // a lane 16 bytes; D / 8 lanes a row
       const int c = lane % (D / 8);
       for (int r = lane / (D / 8); r < kTilesHalf; r += 256 / D) {
@@ -362,10 +434,39 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
           *reinterpret_cast<uint4 *>(to) = load8<false>(q);
       }
       cp_async_commit();
+      const int first = w.first(), count = w.count(S);
+      bool hole = false;   // whether a page of the piece's blocks is missing
+      for (int p = 2 * first + lane; p < 2 * (first + count); p += 32)
+        hole |= p * kPage < w.e.length && page_of(A.pool, w.e.slot, p) < 0;
+      hole = __any_sync(0xffffffffu, hole) != 0;
+      if (lane == 0) {
+        info.count = count;
+        info.first = first;
+        info.base = base;
+        info.packed = packed;
+        info.row0 = w.e.row0;
+        info.n = w.e.n;
+        info.length = w.e.length;
+        info.slot = w.e.slot;
+        info.head = w.head;
+        info.two = halves() == 2;
+        info.whole = w.whole();
+        info.opens = w.opens();
+        info.hole = hole;
+        if (!w.whole()) {
+          info.c0 = piece_of(total, pieces, w.tile_u + S.extra);
+          info.c1 = piece_of(total, pieces, w.tile_u + w.units - 1);
+        }
+      }
       cp_async_wait_all();
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_count(&bars.q_full[h], 1);
+      if (lane == 0) {
+        mbar_arrive_count(&bars.q_full[h][buf], 1);
+        mbar_arrive_count(&bars.i_full[h][n % kInfoSlots], 1);
+      }
+      ++n;
+      more = w.next(A.pool, A.batch, S, line);
     }
   }
   } else {
@@ -376,31 +477,30 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     const uint32_t t_s = tmem + Z::kS + h * 128 + lanes, t_o = tmem + Z::kO + h * D + lanes,
                    t_p = tmem + Z::kP + h * Z::kPHalf + lanes;
     const float c = A.scale_log2;
-    uint32_t steps = 0;   // of this half so far
+    uint32_t steps = 0, n_tiles = 0;   // of this half so far
     bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t phase) {
       ok = __all_sync(0xffffffffu, ok && t_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
       return ok;
     };
-    for (; more; more = w.next(A.pool, A.batch, S, line)) {
-      if (h >= halves()) continue;
-      const int packed = w.e.n * S.group, row = w.t * kTilesTile + h * kTilesHalf + r;
-      const int first = w.first(), count = w.count(S);
-      const bool in = row < packed;
-      const int i = S.row_of(row), g = row - i * S.group;
-      const int pos = in ? w.e.length - w.e.n + i : -1;
-      // whether every page of the piece's blocks is there
-      bool hole = false;
-      for (int x = r; x < 2 * count; x += 128) {
-        const int p = 2 * first + x;
-        hole |= p * kPage < w.e.length && page_of(A.pool, w.e.slot, p) < 0;
-      }
-      hole = half_any(h, hole);
+    uint32_t n_syncs = 0;
+    auto half_sync = [&]() {   // with a limit, as every wait here
+      __syncwarp();
+      if (lane == 0) mbar_arrive_count(&bars.half[h], 1);
+      return wait(&bars.half[h], n_syncs++);
+    };
+    while (true) {
+      if (!wait(&bars.i_full[h][n_tiles % kInfoSlots], n_tiles / kInfoSlots)) break;
+      const TileInfo &info = s_info[h][n_tiles % kInfoSlots];
+      const int first = info.first, count = info.count;
+      if (count == 0) break;
+      ++n_tiles;
+      const int row = info.base + r, i = S.row_of(row), before = info.length - info.n;   // positions before the rows
+      const bool in = row < info.packed, hole = info.hole != 0;
+      const int pos = in ? before + i : -1;
       // positions that every row of the half sees need no mask
-      const int lead = S.row_of(w.t * kTilesTile + h * kTilesHalf);
-      const int tail = S.row_of(min(packed, w.t * kTilesTile + (h + 1) * kTilesHalf) - 1);
-      const int all_hi = w.e.length - w.e.n + lead;
-      const int all_lo = S.window > 0 ? w.e.length - w.e.n + tail - S.window + 1 : 0;
+      const int all_hi = before + S.row_of(info.base);
+      const int all_lo = S.window > 0 ? before + S.row_of(min(info.packed, info.base + kTilesHalf) - 1) - S.window + 1 : 0;
 
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < count; ++j, ++steps) {
@@ -417,17 +517,28 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         }
         const int j0 = (first + j) * kTilesBlock;
         if (hole || j0 + kTilesBlock - 1 > all_hi || j0 < all_lo) {
-          const int hi = pos - j0, lo = S.window > 0 ? hi - S.window : -1;   // sees lo < x <= hi
-          const bool p0 = !hole || page_of(A.pool, w.e.slot, 2 * (first + j)) >= 0;
-          const bool p1 = !hole || page_of(A.pool, w.e.slot, 2 * (first + j) + 1) >= 0;
+          int hi = pos - j0;   // sees x <= hi
+          if (hole || S.window > 0) {
+            int lo = S.window > 0 ? hi - S.window : -1;   // and x > lo
+            if (hole) {
+              if (page_of(A.pool, info.slot, 2 * (first + j)) < 0) lo = max(lo, 63);
+              if (page_of(A.pool, info.slot, 2 * (first + j) + 1) < 0) hi = min(hi, 63);
+            }
+#pragma unroll
+            for (int x = 0; x < 128; ++x)
+              if (x <= lo) s[x] = -INFINITY;
+          }
 #pragma unroll
           for (int x = 0; x < 128; ++x)
-            if (x > hi || x <= lo || !(x < 64 ? p0 : p1)) s[x] = -INFINITY;
+            if (x > hi) s[x] = -INFINITY;
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int x = 4; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        for (int x = 4; x < 124; x += 8) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) mx[y] = max3(mx[y], s[x + y], s[x + 4 + y]);
+        }
+        const float top = max3(max3(mx[0], s[124], s[125]), max3(mx[1], s[126], s[127]), fmaxf(mx[2], mx[3]));
         if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {   // also from m = -inf; both -inf: NaN, no
           const float nm = fmaxf(m, top), a = nm == -INFINITY ? 1.f : exp2_approx((m - nm) * c);
           m = nm;
@@ -450,37 +561,50 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
           if (j > 0 && !wait(&bars.o_done[h], steps - 1)) break;
         }
         const float mc = m == -INFINITY ? 0.f : m * c;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // sixteen exponentials in flight while the sixteen before them are
+        // added up and packed
+        const uint64_t c2 = f2(c, c), mc2 = f2(-mc, -mc);
+        uint64_t sum[4] = {0, 0, 0, 0};
+        uint32_t p[32];
+        float e[2][16];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          uint32_t p[32];
+        for (int x = 0; x <= 8; ++x) {
+          if (x < 8) {
 #pragma unroll
-          for (int y = 0; y < 32; ++y) {
-            const float a = exp2_approx(fmaf(s[x * 64 + 2 * y], c, -mc));
-            const float b = exp2_approx(fmaf(s[x * 64 + 2 * y + 1], c, -mc));
-            sum[(2 * y) & 3] += a;
-            sum[(2 * y + 1) & 3] += b;
-            p[y] = E::pack(a, b);
+            for (int y = 0; y < 8; ++y)
+              f2_split(f2_fma(f2(s[x * 16 + 2 * y], s[x * 16 + 2 * y + 1]), c2, mc2), s[x * 16 + 2 * y], s[x * 16 + 2 * y + 1]);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) e[x & 1][y] = exp2_approx(s[x * 16 + y]);
           }
-          t_st32(t_p + x * 32, p);
+          if (x > 0) {
+            const float *d = e[(x - 1) & 1];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              sum[y & 3] = f2_add(sum[y & 3], f2(d[2 * y], d[2 * y + 1]));
+              p[((x - 1) & 3) * 8 + y] = E::pack(d[2 * y], d[2 * y + 1]);
+            }
+            if (x == 4) t_st32(t_p, p);
+            if (x == 8) t_st32(t_p + 32, p);
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float l0, l1;
+        f2_split(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])), l0, l1);
+        l += l0 + l1;
         t_st_wait();
         t_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_count(&bars.p_full[h], 1);
       }
-      if (ok) wait(&bars.o_done[h], steps - 1);
+      if (!wait(&bars.o_done[h], steps - 1)) break;   // or a wait above gave up: the control block says which
       t_after();
-      const bool whole = w.whole();
+      const bool whole = info.whole != 0;
       constexpr int64_t kTwo = 2 * Z::kPartFloats;   // a part has two halves
-      if (half_any(h, !ok)) break;   // a wait gave up: the control block says which
       bool write = in;
       int c0 = 0, c1 = -1;
       if (!whole) {
         // a tile that other pieces share: leave this part, and the last of
         // them to arrive joins all parts in order; [D / 4][128] of 4 floats
-        float *part = A.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (w.opens() ? 1 : 0)) * kTwo + h * Z::kPartFloats;
+        float *part = A.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (info.opens ? 1 : 0)) * kTwo + h * Z::kPartFloats;
 #pragma unroll
         for (int x = 0; x < D / 32; ++x) {
           float o[32];
@@ -494,16 +618,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         __stcg(part + 128 * D + r, m);
         __stcg(part + 128 * (D + 1) + r, l);
         __threadfence();
-        half_any(h, false);
-        c0 = piece_of(total, pieces, w.tile_u + S.extra);
-        c1 = piece_of(total, pieces, w.tile_u + w.units - 1);
+        if (!half_sync()) break;   // the half's part is written
+        c0 = info.c0;
+        c1 = info.c1;
         if (r == 0) {
           const int before = atomicAdd(&A.arrived[2 * c0 + h], 1);
           s_last[h] = before == c1 - c0;
           if (s_last[h]) A.arrived[2 * c0 + h] = 0;
         }
-        half_any(h, false);
+        if (!half_sync()) break;
         write = write && s_last[h] != 0;
+        if (!half_sync()) break;   // s_last is read
         if (write) {
           __threadfence();
           const float *p = A.parts + h * Z::kPartFloats + 128 * D + r;
@@ -516,10 +641,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
           }
         }
       }
-      bool bad = false;
+      const int g = row - i * S.group, qh = info.head * S.group + g;
+      const int64_t orow = info.row0 + i;
+      if (write && A.lse != nullptr)
+        A.lse[orow * A.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, A.scale, log2_approx(l) * 0.6931471805599453f);
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      T *out = static_cast<T *>(A.out) + (w.e.row0 + i) * A.o_row + (w.head * S.group + g) * A.o_head;
-#pragma unroll 1
+      T *out = static_cast<T *>(A.out) + orow * A.o_row + qh * A.o_head;
+      uint64_t wrong = 0;   // NaN as soon as a value is not finite
+#pragma unroll
       for (int x = 0; x < D / 32; ++x) {
         float o[32];
         if (whole) {
@@ -543,34 +672,40 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
           }
         }
         if (write) {
+          uint32_t u[16];
 #pragma unroll
-          for (int y = 0; y < 32; ++y) {
-            o[y] = l == 0.f ? 0.f : o[y] * inv;
-            bad |= !(fabsf(o[y]) <= 3.4e38f);
+          for (int y = 0; y < 16; ++y) {
+            const uint64_t v = f2_mul(f2(o[2 * y], o[2 * y + 1]), f2(inv, inv));
+            wrong = f2_fma(v, 0, wrong);
+            float a, b;
+            f2_split(v, a, b);
+            u[y] = E::pack(a, b);
           }
+          uint16_t *dst = reinterpret_cast<uint16_t *>(out) + x * 32;
+          if (A.o_wide) {
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const uint4 v = make_uint4(E::pack(o[8 * y], o[8 * y + 1]), E::pack(o[8 * y + 2], o[8 * y + 3]),
-                                       E::pack(o[8 * y + 4], o[8 * y + 5]), E::pack(o[8 * y + 6], o[8 * y + 7]));
-            uint16_t *dst = reinterpret_cast<uint16_t *>(out) + x * 32 + y * 8;
-            if (A.o_vec) store8<true>(dst, v); else store8<false>(dst, v);
+            for (int y = 0; y < 2; ++y) store32(dst + y * 16, u + y * 8);
+          } else {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const uint4 v = make_uint4(u[4 * y], u[4 * y + 1], u[4 * y + 2], u[4 * y + 3]);
+              if (A.o_vec) store8<true>(dst + y * 8, v); else store8<false>(dst + y * 8, v);
+            }
           }
         }
       }
-      if (write && A.lse != nullptr)
-        A.lse[static_cast<int64_t>(w.e.row0 + i) * A.q_heads + w.head * S.group + g] =
-            l == 0.f ? -INFINITY : m * A.scale + logf(l);
       t_before();   // this half's O is read: its next p arrival says so
       // rows with infinities or NaN: each again, alone, by its own warp
-      unsigned again = __ballot_sync(0xffffffffu, bad);
+      float w0, w1;
+      f2_split(wrong, w0, w1);
+      unsigned again = __ballot_sync(0xffffffffu, w0 + w1 != 0.f);
       while (again) {
         const int x = __ffs(again) - 1;
         again &= again - 1;
-        const int y = w.t * kTilesTile + h * kTilesHalf + (warp & 3) * 32 + x;
+        const int y = info.base + (warp & 3) * 32 + x, yi = S.row_of(y);
         __syncwarp();
-        row_alone<D, T>(A, w.e, w.head, y / S.group, y % S.group);
+        row_alone<D, T>(A, Entry{info.row0, info.n, info.length, info.slot}, info.head, yi, y - yi * S.group);
       }
-      half_any(h, false);   // s_last may be written again
     }
   }
   __syncwarp();
