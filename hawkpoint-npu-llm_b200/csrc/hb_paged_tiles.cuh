@@ -31,6 +31,7 @@ namespace paged {
 
 constexpr int kTilesTile = 256, kTilesHalf = 128, kTilesBlock = 128;
 constexpr int kTilesExtra = 2;   // a tile's start and end, in blocks
+constexpr int kTurnAt = 5;   // of eight parts of its exponentials, those a half has added up when it passes its turn on
 constexpr int kTilesThreads = 384;
 // Registers a thread after the split: 256 softmax threads x 216 + 128 others x
 // 72 = 384 x 168, what the block is launched with.
@@ -59,20 +60,33 @@ __device__ __forceinline__ void t_dealloc(uint32_t taddr, uint32_t ncols) {
 }
 __device__ __forceinline__ void t_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void t_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void t_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+// The MMA warp's instructions are issued by one lane (`leader` nonzero in
+// one) as predicated instructions in code that all lanes run: their operands
+// live in uniform registers, and a branch of one lane would have each of them
+// moved there anew (eight MMAs took 650 cycles to issue).
+__device__ __forceinline__ uint32_t t_leader() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void t_commit(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(bar), "r"(leader) : "memory");
 }
 // D[tmem] (+)= A[smem] B[smem], and A[tmem] B[smem]
-__device__ __forceinline__ void t_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+__device__ __forceinline__ void t_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                                         uint32_t leader) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader) : "memory");
 }
-__device__ __forceinline__ void t_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+__device__ __forceinline__ void t_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                                         uint32_t leader) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader) : "memory");
 }
 // 32 consecutive 32-bit columns of this thread's TMEM lane.
 __device__ __forceinline__ void t_ld32(uint32_t taddr, float *r) {
@@ -194,6 +208,7 @@ struct TilesBars {
   uint64_t s_full[2], s_read[2], p_full[2], o_done[2];
   uint64_t i_full[2][kInfoSlots];                          // a tile is told: what the softmax, which MMAs of
                                                            // short tiles may run ahead of, waits for
+  uint64_t turn[2][4];                                     // the exponentials are free for a half's warp
   uint64_t half[2];                                        // a half's four softmax warps
   uint64_t done;
 };
@@ -229,6 +244,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       mbar_init(&bars.p_full[h], 4);
       mbar_init(&bars.o_done[h], 1);
       mbar_init(&bars.half[h], 4);
+      for (int x = 0; x < 4; ++x) mbar_init(&bars.turn[h][x], 1);
       for (int x = 0; x < kInfoSlots; ++x) mbar_init(&bars.i_full[h][x], 1);
     }
     mbar_init(&bars.done, 1);
@@ -242,7 +258,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   t_before();
   __syncthreads();
   t_after();
-  const uint32_t tmem = s_tmem;
+  // 512 columns are all of them: the allocation starts at column 0
 
   Walk w;
   w.u = piece_begin(total, pieces, blockIdx.x);
@@ -309,90 +325,101 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     for (int i = max(0, it - Z::kStages); i < it; ++i)   // nothing in flight when the block ends
       mbar_wait_quiet(&bars.full[i % Z::kStages], static_cast<uint32_t>(i / Z::kStages) & 1u, A.limit_ns);
   } else if (warp == 8) {
-    // ---- MMA issue: the warp walks, its first lane issues
+    // ---- MMA issue
     constexpr uint32_t kIdescS = tiles_idesc<T>(kTilesBlock, false), kIdescO = tiles_idesc<T>(D, true);
-    int it = 0;                                  // ring stages consumed
-    uint32_t n_q[2] = {0, 0}, n_s[2] = {0, 0};   // tiles and steps of either half so far
-    bool ok = true;
     constexpr uint32_t kStep = Z::kOperand >> 4;
+    const uint32_t leader = t_leader();
     const uint32_t q_lo = swizzled_lo(smem_u32(smem), 16), k_lo = swizzled_lo(smem_u32(ring), 16),
                    v_lo = swizzled_lo(smem_u32(ring), 16384);
+    uint32_t it = 0;                // ring stages consumed
+    uint32_t n_q0 = 0, n_q1 = 0, n_s0 = 0, n_s1 = 0;   // tiles and steps of either half so far
+    bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t phase) {
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
+      ok = __all_sync(0xffffffffu, ok && t_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
       return ok;
     };
-    auto stage = [&](int i) { return i % Z::kStages; };
-    auto wait_ring = [&](int i) { return wait(&bars.full[stage(i)], static_cast<uint32_t>(i / Z::kStages)); };
-    auto commit = [&](uint64_t *bar) {
-      if (lane == 0) t_commit(bar);
-    };
-    auto mma_s = [&](int h, int i) {   // S of half h from the K in ring use i
+    auto stage = [&](uint32_t i) { return i % Z::kStages; };
+    auto wait_ring = [&](uint32_t i) { return wait(&bars.full[stage(i)], i / Z::kStages); };
+    auto commit = [&](uint64_t *bar) { t_commit(smem_u32(bar), leader); };
+    // S of half h from its q buffer and the K in ring use i
+    auto mma_s = [&](int h, uint32_t buf, uint32_t i) {
       t_after();
-      const uint32_t a = q_lo + ((n_q[h] - 1) % Z::kQ * 2 + h) * kStep, b = k_lo + stage(i) * kStep;
-      if (lane == 0) {
+      const uint32_t a = q_lo + (buf * 2 + h) * kStep, b = k_lo + stage(i) * kStep;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-          t_mma_ss(tmem + Z::kS + h * 128, swizzled_desc(a + off), swizzled_desc(b + off), kIdescS, k != 0);
-        }
-        t_commit(&bars.s_full[h]);
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+        t_mma_ss(Z::kS + h * 128, swizzled_desc(a + off), swizzled_desc(b + off), kIdescS, k != 0, leader);
       }
+      commit(&bars.s_full[h]);
     };
-    auto mma_o = [&](int h, int i, bool fresh) {   // O of half h from the V in ring use i
+    // O of half h from its P and the V in ring use i
+    auto mma_o = [&](int h, uint32_t i, uint32_t acc) {
       t_after();
       const uint32_t b = v_lo + stage(i) * kStep;
-      if (lane == 0) {
 #pragma unroll
-        for (int k = 0; k < kTilesBlock / 16; ++k)
-          t_mma_ts(tmem + Z::kO + h * D, tmem + Z::kP + h * Z::kPHalf + k * 8, swizzled_desc(b + k * (2048 >> 4)),
-                   kIdescO, !(fresh && k == 0));
-        t_commit(&bars.o_done[h]);
-      }
+      for (int k = 0; k < kTilesBlock / 16; ++k)
+        t_mma_ts(Z::kO + h * D, Z::kP + h * Z::kPHalf + k * 8, swizzled_desc(b + k * (2048 >> 4)), kIdescO, k ? 1 : acc,
+                 leader);
+      commit(&bars.o_done[h]);
     };
     while (ok) {
-      if (!wait(&bars.q_full[0][n_q[0] % Z::kQ], n_q[0] / Z::kQ)) break;
-      const TileInfo &info = s_info[0][n_q[0] % kInfoSlots];
-      const int count = info.count, nh = info.two ? 2 : 1;
+      const uint32_t buf0 = n_q0 % Z::kQ;
+      if (!wait(&bars.q_full[0][buf0], n_q0 / Z::kQ)) break;
+      const TileInfo &info = s_info[0][n_q0 % kInfoSlots];
+      // reductions over the warp, for results in uniform registers
+      const uint32_t count = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(info.count));
+      const bool two = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(info.two)) != 0;
       if (count == 0) break;
       // S is free: the last step's P of either half, which was waited for,
       // was written after its S was read
-      ++n_q[0];
-      if (nh == 2) {
-        wait(&bars.q_full[1][n_q[1] % Z::kQ], n_q[1] / Z::kQ);
-        ++n_q[1];
+      ++n_q0;
+      const uint32_t buf1 = n_q1 % Z::kQ;
+      if (two) {
+        wait(&bars.q_full[1][buf1], n_q1 / Z::kQ);
+        ++n_q1;
       }
       if (!wait_ring(it)) break;
-      for (int h = 0; h < nh; ++h) mma_s(h, it);
+      mma_s(0, buf0, it);
+      if (two) mma_s(1, buf1, it);
       commit(&bars.empty[stage(it)]);
-      if (count == 1)
-        for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h][(n_q[h] - 1) % Z::kQ]);
-      for (int j = 0; j < count && ok; ++j) {
+      for (uint32_t j = 0; j < count; ++j) {
         const bool next = j + 1 < count;
-        const int ik = it + 2 * j + 1, iv = next ? ik + 1 : ik;
+        const uint32_t ik = it + 2 * j + 1, iv = next ? ik + 1 : ik;
+        if (!next) {   // every S of the tile is issued
+          commit(&bars.q_empty[0][buf0]);
+          if (two) commit(&bars.q_empty[1][buf1]);
+        }
         if (next && !wait_ring(ik)) break;
         if constexpr (Z::kEarly) {
           if (next) {
-            for (int h = 0; h < nh; ++h)
-              if (wait(&bars.s_read[h], n_s[h])) mma_s(h, ik);
+            if (!wait(&bars.s_read[0], n_s0)) break;
+            mma_s(0, buf0, ik);
+            if (two) {
+              if (!wait(&bars.s_read[1], n_s1)) break;
+              mma_s(1, buf1, ik);
+            }
             commit(&bars.empty[stage(ik)]);
-            if (j + 2 == count)
-              for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h][(n_q[h] - 1) % Z::kQ]);
           }
           if (!wait_ring(iv)) break;
-          for (int h = 0; h < nh; ++h)
-            if (wait(&bars.p_full[h], n_s[h]++)) mma_o(h, iv, j == 0);
+          if (!wait(&bars.p_full[0], n_s0++)) break;
+          mma_o(0, iv, j != 0);
+          if (two) {
+            if (!wait(&bars.p_full[1], n_s1++)) break;
+            mma_o(1, iv, j != 0);
+          }
           commit(&bars.empty[stage(iv)]);
         } else {
           if (!wait_ring(iv)) break;
-          for (int h = 0; h < nh; ++h)
-            if (wait(&bars.p_full[h], n_s[h]++)) {
-              mma_o(h, iv, j == 0);
-              if (next) mma_s(h, ik);   // over the P just used: MMAs run in order
-            }
+          if (!wait(&bars.p_full[0], n_s0++)) break;
+          mma_o(0, iv, j != 0);
+          if (next) mma_s(0, buf0, ik);   // over the P just used: MMAs run in order
+          if (two) {
+            if (!wait(&bars.p_full[1], n_s1++)) break;
+            mma_o(1, iv, j != 0);
+            if (next) mma_s(1, buf1, ik);
+          }
           if (next) commit(&bars.empty[stage(ik)]);
           commit(&bars.empty[stage(iv)]);
-          if (j + 2 == count)
-            for (int h = 0; h < nh; ++h) commit(&bars.q_empty[h][(n_q[h] - 1) % Z::kQ]);
         }
       }
       it += 2 * count;
@@ -474,10 +501,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     // ---- softmax of half h, a thread a row
     const int h = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + Z::kS + h * 128 + lanes, t_o = tmem + Z::kO + h * D + lanes,
-                   t_p = tmem + Z::kP + h * Z::kPHalf + lanes;
+    const uint32_t t_s = Z::kS + h * 128 + lanes, t_o = Z::kO + h * D + lanes,
+                   t_p = Z::kP + h * Z::kPHalf + lanes;
     const float c = A.scale_log2;
     uint32_t steps = 0, n_tiles = 0;   // of this half so far
+    uint32_t turns = 0;                // steps of tiles with two halves
     bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t phase) {
       ok = __all_sync(0xffffffffu, ok && t_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
@@ -495,6 +523,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       const int first = info.first, count = info.count;
       if (count == 0) break;
       ++n_tiles;
+      const bool two = info.two != 0;
       const int row = info.base + r, i = S.row_of(row), before = info.length - info.n;   // positions before the rows
       const bool in = row < info.packed, hole = info.hole != 0;
       const int pos = in ? before + i : -1;
@@ -560,6 +589,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         if constexpr (Z::kEarly) {   // P is free when the last step's P V has read it
           if (j > 0 && !wait(&bars.o_done[h], steps - 1)) break;
         }
+        // The halves take turns at the exponentials: left alone they run them at
+        // the same time, at half speed each, and then both wait at the same time.
+        if (two && !wait(&bars.turn[h][warp & 3], turns - (h == 0 ? 1 : 0))) break;
         const float mc = m == -INFINITY ? 0.f : m * c;
         // sixteen exponentials in flight while the sixteen before them are
         // added up and packed
@@ -584,9 +616,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
               p[((x - 1) & 3) * 8 + y] = E::pack(d[2 * y], d[2 * y + 1]);
             }
             if (x == 4) t_st32(t_p, p);
+            if (x == kTurnAt && two && lane == 0) mbar_arrive_count(&bars.turn[h ^ 1][warp & 3], 1);
             if (x == 8) t_st32(t_p + 32, p);
           }
         }
+        turns += two ? 1 : 0;
         float l0, l1;
         f2_split(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])), l0, l1);
         l += l0 + l1;
@@ -714,7 +748,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   t_before();
   __syncthreads();
   t_after();
-  if (warp == 0) t_dealloc(tmem, 512);
+  if (warp == 0) t_dealloc(s_tmem, 512);
 }
 
 }  // namespace paged

@@ -27,11 +27,19 @@ streams with events.
 """
 
 import ctypes
-import math
+import struct
 
 from runtime import hb_lib
 
 PAGE = 64
+
+# The structs of a call, filled in place: a decode step makes tens of calls, and
+# building ctypes objects for each would cost more than the launches.
+_ROWS = struct.Struct("=QQiiii")            # hb_paged_rows
+_QUERY = struct.Struct("=QqqQqqQiifi")      # hb_paged_query
+_NEW = struct.Struct("=QqQqqQQii")          # hb_paged_new
+assert (_ROWS.size, _QUERY.size, _NEW.size) == tuple(
+    ctypes.sizeof(c) for c in (hb_lib.HbPagedRows, hb_lib.HbPagedQuery, hb_lib.HbPagedNew))
 
 
 def _torch():
@@ -102,43 +110,55 @@ class PagedKVCache:
         self._workspace = torch.zeros(need, dtype=torch.uint8, device=pool.device)
         p.workspace_dev, p.workspace_bytes = self._workspace.data_ptr(), need
         self._index = pool.device.index if pool.device.index is not None else torch.cuda.current_device()
+        self._int32, self._float32 = torch.int32, torch.float32
+        self._scale = self.head_dim ** -0.5
+        self._empty = torch.empty_strided
+        self._current_device = torch.cuda.current_device
+        # torch's own accessor of the current stream's handle, without a Stream object where there is one
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._current_stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+        # what a call fills, and its addresses
+        self._rows_buf, self._args_buf = bytearray(_ROWS.size), bytearray(max(_QUERY.size, _NEW.size))
+        self._rows_at, self._args_at = (ctypes.addressof(ctypes.c_char.from_buffer(b)) for b in (self._rows_buf, self._args_buf))
 
     # -- helpers -----------------------------------------------------------------
-    def _stream(self):
-        return _torch().cuda.current_stream(self._index).cuda_stream
-
     def _call(self, fn, *args):
-        torch = _torch()
-        if torch.cuda.current_device() == self._index:
-            rc = fn(self._pool, *args, self._stream())
+        if self._current_device() == self._index:
+            rc = fn(self._pool, *args, self._current_stream(self._index))
         else:
-            with torch.cuda.device(self._index):
-                rc = fn(self._pool, *args, self._stream())
+            with _torch().cuda.device(self._index):
+                rc = fn(self._pool, *args, self._current_stream(self._index))
         if rc:
             hb_lib.check(rc)
 
     def _list(self, name, t, n=None):
-        if t.dtype != _torch().int32 or t.dim() != 1 or not t.is_contiguous() or t.device != self.device:
+        if t.dtype is not self._int32 or t.dim() != 1 or not t.is_contiguous() or t.device != self.device:
             raise ValueError(f"{name} must be a contiguous one-dimensional int32 tensor on the cache's device")
         if n is not None and t.shape[0] != n:
             raise ValueError(f"{name} has {t.shape[0]} entries, not {n}")
         return t.data_ptr()
 
-    def _rows(self, slots, row_start, rows, max_rows):
+    def _fill_rows(self, slots, row_start, rows, max_rows):
         entries = slots.shape[0]
         if max_rows < 0 or (entries == 0 and rows > 0):
             raise ValueError("max_rows must not be negative, and rows need an entry")
-        return hb_lib.HbPagedRows(self._list("slots", slots), self._list("row_start", row_start, entries + 1), entries,
-                                  rows, min(int(max_rows), rows), 0)
+        _ROWS.pack_into(self._rows_buf, 0, self._list("slots", slots), self._list("row_start", row_start, entries + 1),
+                        entries, rows, max_rows if max_rows < rows else rows, 0)
 
     def _heads(self, name, t, rows=None):
-        if t.dim() != 3 or t.dtype != self.dtype or t.device != self.device or t.shape[2] != self.head_dim or (
-                t.stride(2) != 1):
-            raise ValueError(f"{name} must be [rows, heads, {self.head_dim}] of {self.dtype} on the cache's device, "
-                             "its last dimension contiguous")
-        if rows is not None and tuple(t.shape[:2]) != rows:
-            raise ValueError(f"{name} of shape {tuple(t.shape)}: must be {rows + (self.head_dim,)}")
-        return t
+        """(shape, strides) of rows of heads."""
+        if t.dtype is not self.dtype or t.dim() != 3 or t.device != self.device:
+            raise ValueError(f"{name} must be [rows, heads, {self.head_dim}] of {self.dtype} on the cache's device")
+        shape, stride = t.shape, t.stride()
+        if shape[2] != self.head_dim or stride[2] != 1:
+            raise ValueError(f"{name} of shape {tuple(shape)}: its last dimension must be {self.head_dim}, contiguous")
+        if rows is not None and shape[:2] != rows:
+            raise ValueError(f"{name} of shape {tuple(shape)}: must be {tuple(rows) + (self.head_dim,)}")
+        return shape, stride
+
+    def _new_heads(self, rows, heads):
+        d = self.head_dim
+        return self._empty((rows, heads, d), (heads * d, d, 1), dtype=self.dtype, device=self.device)
 
     # -- rows ----------------------------------------------------------------------
     def append(self, layer, qkv, slots, row_start, max_rows, cos, sin, out=None):
@@ -146,28 +166,29 @@ class PagedKVCache:
         the slots' pages (``reserve`` has mapped them).  ``qkv`` [rows, (q
         heads + 2 kv heads) * head_dim]; ``cos`` / ``sin`` float32 [positions,
         head_dim / 2].  Returns the rotated q [rows, q heads, head_dim]."""
-        torch = _torch()
         d = self.head_dim
-        if qkv.dim() != 2 or qkv.dtype != self.dtype or qkv.device != self.device or qkv.stride(1) != 1 or qkv.shape[1] % d:
-            raise ValueError(f"qkv must be [rows, heads * {d}] of {self.dtype} on the cache's device, its last "
-                             "dimension contiguous")
-        rows, q_heads = int(qkv.shape[0]), int(qkv.shape[1]) // d - 2 * self.kv_heads
+        if qkv.dtype is not self.dtype or qkv.dim() != 2 or qkv.device != self.device:
+            raise ValueError(f"qkv must be [rows, heads * {d}] of {self.dtype} on the cache's device")
+        (rows, cols), (row_stride, col_stride) = qkv.shape, qkv.stride()
+        if cols % d or col_stride != 1:
+            raise ValueError(f"qkv of shape {tuple(qkv.shape)}: its rows must be whole heads of {d}, contiguous")
+        q_heads = cols // d - 2 * self.kv_heads
         if q_heads < 0:
             raise ValueError(f"qkv has fewer heads than the {2 * self.kv_heads} of k and v")
+        table = cos.shape
         for name, t in (("cos", cos), ("sin", sin)):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] * 2 != d or not t.is_contiguous() or (
-                    t.device != self.device):
-                raise ValueError(f"{name} must be a contiguous float32 [positions, {d // 2}] on the cache's device")
-        if cos.shape != sin.shape:
-            raise ValueError("cos and sin must have the same shape")
+            if t.dtype is not self._float32 or t.shape != table or len(table) != 2 or table[1] * 2 != d or (
+                    not t.is_contiguous() or t.device != self.device):
+                raise ValueError(f"{name} must be a contiguous float32 [positions, {d // 2}] on the cache's device, "
+                                 "cos and sin of one shape")
         if out is None:
-            out = torch.empty((rows, q_heads, d), dtype=self.dtype, device=self.device)
+            out, q_row, q_head = self._new_heads(rows, q_heads), q_heads * d, d
         else:
-            self._heads("out", out, (rows, q_heads))
-        r = self._rows(slots, row_start, rows, max_rows)
-        n = hb_lib.HbPagedNew(qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), out.stride(1),
-                              cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_heads)
-        self._call(self._lib.hb_paged_append, layer, ctypes.byref(r), ctypes.byref(n))
+            _, (q_row, q_head, _) = self._heads("out", out, (rows, q_heads))
+        self._fill_rows(slots, row_start, rows, max_rows)
+        _NEW.pack_into(self._args_buf, 0, qkv.data_ptr(), row_stride, out.data_ptr(), q_row, q_head, cos.data_ptr(),
+                       sin.data_ptr(), table[0], q_heads)
+        self._call(self._lib.hb_paged_append, layer, self._rows_at, self._args_at)
         return out
 
     def attend(self, layer, q, slots, row_start, max_rows, scale=None, window=0, out=None, lse=False):
@@ -176,19 +197,16 @@ class PagedKVCache:
         ``window`` of them); ``scale`` defaults to 1 / sqrt(head_dim).  Returns
         the output in q's shape; with ``lse`` also float32 [rows, q heads], the
         log of the sum of exp(scores).  Rows that see nothing give 0 and -inf."""
-        torch = _torch()
-        self._heads("q", q)
-        rows, q_heads = int(q.shape[0]), int(q.shape[1])
+        (rows, heads, d), (q_row, q_head, _) = self._heads("q", q)
         if out is None:
-            out = torch.empty((rows, q_heads, self.head_dim), dtype=self.dtype, device=self.device)
+            out, o_row, o_head = self._new_heads(rows, heads), heads * d, d
         else:
-            self._heads("out", out, (rows, q_heads))
-        sums = torch.empty((rows, q_heads), dtype=torch.float32, device=self.device) if lse else None
-        r = self._rows(slots, row_start, rows, max_rows)
-        a = hb_lib.HbPagedQuery(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                                sums.data_ptr() if lse else None, q_heads, window,
-                                1.0 / math.sqrt(self.head_dim) if scale is None else scale, 0)
-        self._call(self._lib.hb_paged_attend, layer, ctypes.byref(r), ctypes.byref(a))
+            _, (o_row, o_head, _) = self._heads("out", out, (rows, heads))
+        sums = self._empty((rows, heads), (heads, 1), dtype=self._float32, device=self.device) if lse else None
+        self._fill_rows(slots, row_start, rows, max_rows)
+        _QUERY.pack_into(self._args_buf, 0, q.data_ptr(), q_row, q_head, out.data_ptr(), o_row, o_head,
+                         sums.data_ptr() if lse else 0, heads, window, self._scale if scale is None else scale, 0)
+        self._call(self._lib.hb_paged_attend, layer, self._rows_at, self._args_at)
         return (out, sums) if lse else out
 
     # -- pages -----------------------------------------------------------------------
