@@ -179,15 +179,20 @@ int launch_copy(const hb_page_pool &p, void *to_pages, int to_n, const int *from
 }
 
 // Which kernels an attention call launches: the rows kernel for entries of up
-// to 16 packed rows, the tiles kernel for the others, one of them where the
-// bound on an entry's rows (or, all being equal, their sum) says that it has
-// nothing to leave to the other.  A bound that is wrong costs time, not rows:
-// a kernel launched alone takes every entry.
+// to 16 packed rows (its tile), the tiles kernel for the others, one of them
+// where the host's numbers say that it may have them all.  Where entries have
+// no more than a 16-row tile each on average and none is long, a second launch
+// costs more than the rows kernel loses on the few that have more (96 streams,
+// 12 of them with chunks of up to 32 x 3 packed rows: 37 us in one launch, 56
+// in two); all entries alike above 16 rows are the tiles kernel's.  A bound on
+// an entry's rows that is wrong costs time, not rows: a kernel launched alone
+// takes every entry.
 template <int D, class T>
 cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) {
   const pg::Batch &b = A.batch;
   const int64_t most = static_cast<int64_t>(max_rows) * A.shape.group;
-  const bool rows_only = most <= pg::kRowsTile;
+  const bool rows_only = most <= pg::kRowsTile ||
+                         (most <= 8 * pg::kRowsTile && static_cast<int64_t>(b.rows) * A.shape.group <= static_cast<int64_t>(b.entries) * pg::kRowsTile);
   const bool tiles_only = !rows_only && static_cast<int64_t>(b.entries) * max_rows == b.rows;
   const size_t line = pg::line_bytes(b.entries);
   A.few = rows_only ? INT32_MAX : tiles_only ? 0 : pg::kRowsTile;
@@ -195,7 +200,7 @@ cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) 
     A.shape.tile = pg::kRowsTile;
     A.shape.block = pg::kPage;
     A.shape.extra = pg::kRowsExtra;
-    pg::paged_rows_kernel<D, T><<<rows_pieces(D, sms), pg::kRowsThreads, pg::RowsSize<D>::kSmem + line, st>>>(A, 2);
+    pg::paged_rows_kernel<D, T><<<rows_pieces(D, sms), pg::kRowsThreads, pg::RowsSize<D>::kSmem + line, st>>>(A, pg::kRowsLeast);
   }
   if (!rows_only) {
     A.shape.tile = pg::kTilesTile;
@@ -203,7 +208,18 @@ cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) 
     A.shape.extra = pg::kTilesExtra;
     A.arrived = A.arrived2;
     A.parts = A.parts2;
-    pg::paged_tiles_kernel<D, T><<<sms, pg::kTilesThreads, pg::TilesSize<D>::kSmem + line, st>>>(A, 4);
+    // beside the rows kernel, whose blocks leave first (it reads nothing of it)
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(sms);
+    cfg.blockDim = dim3(pg::kTilesThreads);
+    cfg.dynamicSmemBytes = pg::TilesSize<D>::kSmem + line;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = tiles_only ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, pg::paged_tiles_kernel<D, T>, A, pg::kTilesLeast);
   }
   return cudaGetLastError();
 }
@@ -262,6 +278,10 @@ int hb_paged_attend(const hb_page_pool *pool, int layer, const hb_paged_rows *ro
   if (!(q->scale > 0.f) || q->scale > 1e30f || q->window < 0)
     return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_attend: scale must be positive, window not negative");
   if (rows->rows == 0 || rows->entries == 0) return HB_OK;
+  // the most units the call's line can have (16-row tiles), counted in 32 bits
+  const double units = (static_cast<double>(rows->rows) * q->q_heads / pg::kRowsTile + pool->kv_heads * rows->entries) *
+                       (pool->table_width + pg::kRowsExtra);
+  if (units >= 2e9) return fail(nullptr, HB_ERR_UNSUPPORTED, "hb_paged_attend: too many rows for the table's width in one call");
   if (!q->q_dev || !q->out_dev) return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_attend: null pointer");
   if ((reinterpret_cast<uintptr_t>(q->q_dev) | reinterpret_cast<uintptr_t>(q->out_dev)) & 1)
     return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_attend: q and out must be element aligned");

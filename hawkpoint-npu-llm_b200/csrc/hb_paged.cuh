@@ -105,14 +105,14 @@ __device__ __forceinline__ int tiles_of(const Shape &S, const Entry &e) { return
 // The line of a call: its entries and prefix[b], the units before entry b, in
 // shared memory.
 struct Line {
-  int64_t *prefix;   // [entries + 1]
+  int *prefix;       // [entries + 1]; the host has checked that the total fits
   Entry *entry;      // [entries]
 };
 __host__ __device__ inline size_t line_bytes(int entries) {
-  return (static_cast<size_t>(entries) * (8 + sizeof(Entry)) + 8 + 15) / 16 * 16;
+  return (static_cast<size_t>(entries) * (4 + sizeof(Entry)) + 4 + 15) / 16 * 16;
 }
 __device__ __forceinline__ Line line_at(uint8_t *smem, int entries) {
-  return Line{reinterpret_cast<int64_t *>(smem + entries * sizeof(Entry)), reinterpret_cast<Entry *>(smem)};
+  return Line{reinterpret_cast<int *>(smem + entries * sizeof(Entry)), reinterpret_cast<Entry *>(smem)};
 }
 
 // Fills the line, by all threads of the block: a thread an entry, so that the
@@ -127,7 +127,7 @@ __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const S
     Entry e{0, 0, 0, -1};
     if (b < B.entries) line.entry[b] = e = entry_of(P, B, b);
     const int tiles = b < B.entries && take(e) ? tiles_of(S, e) : 0;
-    int64_t u = 0;
+    int u = 0;
     if (tiles <= 4)
       for (int t = 0; t < tiles; ++t) u += tile_units(S, e, t);
     for (unsigned many = __ballot_sync(0xffffffffu, tiles > 4); many; many &= many - 1) {
@@ -135,21 +135,20 @@ __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const S
       const Entry y{0, __shfl_sync(0xffffffffu, e.n, x), __shfl_sync(0xffffffffu, e.length, x), 0};
       int v = 0;
       for (int t = lane; t < n; t += 32) v += tile_units(S, y, t);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      v = __reduce_add_sync(0xffffffffu, v);
       if (lane == x) u = v;
     }
     if (b < B.entries) line.prefix[b + 1] = u * P.kv_heads;
   }
   __syncthreads();
   if (warp == 0) {
-    int64_t base = 0;
+    int base = 0;
     for (int b0 = 0; b0 < B.entries; b0 += 32) {
       const int b = b0 + lane;
-      int64_t v = b < B.entries ? line.prefix[b + 1] : 0;
+      int v = b < B.entries ? line.prefix[b + 1] : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
+        const int w = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += w;
       }
       if (b < B.entries) line.prefix[b + 1] = base + v;
@@ -163,8 +162,8 @@ __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const S
 // A walk over the tiles of one piece [u, end) of the line, the same in every
 // lane of the warps that make it.
 struct Walk {
-  int64_t u, end;        // units left
-  int64_t tile_u;        // first unit of the current tile, its extra ones included
+  int u, end;            // units left
+  int tile_u;            // first unit of the current tile, its extra ones included
   int b, head, t, units, tiles, blocks_before;
   Entry e;
   Span span;
@@ -174,12 +173,12 @@ struct Walk {
     span = tile_span(S, e, t);
     units = max(1, span.hi - span.lo) + S.extra;
     // where the piece enters the tile's blocks
-    blocks_before = static_cast<int>(max(static_cast<int64_t>(0), u - tile_u - S.extra));
+    blocks_before = max(0, u - tile_u - S.extra);
   }
   // On the tile that holds unit u; false when the piece is done.
   __device__ __forceinline__ bool start(const Pool &P, const Batch &B, const Shape &S, const Line &line) {
     if (u >= end) return false;
-    const int64_t *prefix = line.prefix;
+    const int *prefix = line.prefix;
     int lo = 0, hi = B.entries - 1;
     while (lo < hi) {  // the entry that holds unit u
       const int mid = (lo + hi) >> 1;
@@ -188,11 +187,11 @@ struct Walk {
     b = lo;
     e = line.entry[b];
     tiles = tiles_of(S, e);
-    int64_t rem = u - prefix[b];
+    int rem = u - prefix[b];
     head = 0;
     if (P.kv_heads > 1) {
-      const int64_t per = (prefix[b + 1] - prefix[b]) / P.kv_heads;
-      head = static_cast<int>(rem / per);
+      const int per = (prefix[b + 1] - prefix[b]) / P.kv_heads;
+      head = rem / per;
       rem -= head * per;
     }
     tile_u = u - rem;
@@ -223,7 +222,7 @@ struct Walk {
   // the piece's blocks of the tile: [first, first + count)
   __device__ __forceinline__ int first() const { return span.lo + blocks_before; }
   __device__ __forceinline__ int count(const Shape &S) const {
-    return static_cast<int>(min(end, tile_u + units) - tile_u) - S.extra - blocks_before;
+    return min(end, tile_u + units) - tile_u - S.extra - blocks_before;
   }
   __device__ __forceinline__ bool opens() const { return blocks_before == 0; }
   __device__ __forceinline__ bool whole() const { return opens() && tile_u + units <= end; }
@@ -252,16 +251,29 @@ struct Walk {
   }
 };
 
-// Piece c of `pieces` equal pieces of [0, total).
-__device__ __forceinline__ int64_t piece_begin(int64_t total, int pieces, int c) {
-  return total * c / pieces;
-}
-// The piece that holds unit u.
-__device__ __forceinline__ int piece_of(int64_t total, int pieces, int64_t u) {
-  int c = static_cast<int>(u * pieces / total);
-  while (c + 1 < pieces && piece_begin(total, pieces, c + 1) <= u) ++c;
-  while (c > 0 && piece_begin(total, pieces, c) > u) --c;
-  return c;
+// The line cut into `pieces` pieces, the first `longer` of them a unit longer.
+struct Cut {
+  int pieces, size, longer;
+  __device__ __forceinline__ Cut(int total, int most, int least) {
+    pieces = min(most, (total + least - 1) / least);
+    size = pieces ? total / pieces : 0;
+    longer = total - size * pieces;
+  }
+  __device__ __forceinline__ int begin(int c) const { return size * c + min(c, longer); }
+  // the piece that holds unit u
+  __device__ __forceinline__ int of(int u) const {
+    const int border = (size + 1) * longer;
+    return u < border ? u / (size + 1) : longer + (u - border) / size;
+  }
+};
+
+// Counts one up and returns what was there, ordered after what the block's
+// threads wrote before the barrier above it and before what they read after
+// the one below it.
+__device__ __forceinline__ int arrive_acq_rel(int *p) {
+  int v;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+  return v;
 }
 
 // ---- elements -------------------------------------------------------------------

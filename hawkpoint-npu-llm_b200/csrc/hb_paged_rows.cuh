@@ -20,7 +20,8 @@ namespace hb {
 namespace paged {
 
 constexpr int kRowsTile = 16;
-constexpr int kRowsExtra = 1;                       // a tile's start and end, in pages
+constexpr int kRowsExtra = 4;                       // a tile's start and end, in pages
+constexpr int kRowsLeast = 5;                       // units a piece has at least
 constexpr int kRowsWarps = 4;                       // consumer warps
 constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
 template <int D>
@@ -119,6 +120,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
   __shared__ int s_valid[Z::kStages];
   __shared__ float s_m[kRowsWarps][kRowsTile], s_l[kRowsWarps][kRowsTile];
   __shared__ int s_bad[kRowsTile], s_last;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the tiles kernel of the same call may start
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Shape S = A.shape;
   const Line line = line_at(smem + Z::kSmem, A.batch.entries);
@@ -133,12 +135,11 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
   }
   if (threadIdx.x < kRowsTile) s_bad[threadIdx.x] = 0;
   fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group <= A.few; });
-  const int64_t total = line.prefix[A.batch.entries];
-  const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + least - 1) / least));
-  if (static_cast<int>(blockIdx.x) >= pieces) return;
+  const Cut cut(line.prefix[A.batch.entries], gridDim.x, least);
+  if (static_cast<int>(blockIdx.x) >= cut.pieces) return;
   Walk w;
-  w.u = piece_begin(total, pieces, blockIdx.x);
-  w.end = piece_begin(total, pieces, blockIdx.x + 1);
+  w.u = cut.begin(blockIdx.x);
+  w.end = cut.begin(blockIdx.x + 1);
   bool more = w.start(A.pool, A.batch, S, line);
   int it = 0;  // stages used so far
 
@@ -344,39 +345,61 @@ __global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_c
           __stcg(part + kRowsTile * (D + 1) + r, tl);
         }
       }
-      __threadfence();
       rows_sync();
-      const int c0 = piece_of(total, pieces, w.tile_u + S.extra);
-      const int c1 = piece_of(total, pieces, w.tile_u + w.units - 1);
+      const int c0 = cut.of(w.tile_u + S.extra), parts = cut.of(w.tile_u + w.units - 1) - c0 + 1;
       if (threadIdx.x == 0) {
-        const int before = atomicAdd(&A.arrived[c0], 1);
-        s_last = before == c1 - c0;
+        s_last = arrive_acq_rel(&A.arrived[c0]) == parts - 1;   // the barriers make it all threads'
         if (s_last) A.arrived[c0] = 0;
       }
       rows_sync();
       write = write && s_last != 0;
-      if (write) {
-        __threadfence();
-        const float *p0 = A.parts + (static_cast<int64_t>(c0) * 2 + 1) * Z::kPartFloats;
-        const float *p1 = A.parts + static_cast<int64_t>(c0 + 1) * 2 * Z::kPartFloats;   // then every 2 parts
-        tm = __ldcg(p0 + kRowsTile * D + r);
-        for (int c = 0; c < c1 - c0; ++c) tm = fmaxf(tm, __ldcg(p1 + c * 2 * Z::kPartFloats + kRowsTile * D + r));
-        const float use = tm == -INFINITY ? 0.f : tm;
+      if (s_last != 0) {
+        // part k: the second slot of the first piece, the first of the others
+        const float *base = A.parts + static_cast<int64_t>(c0) * 2 * Z::kPartFloats;
+        auto part_at = [&](int k) { return base + (static_cast<int64_t>(k) * 2 + (k == 0 ? 1 : 0)) * Z::kPartFloats; };
+        // eight parts a round, all their reads in flight; of the eight threads
+        // of a row each weighs one part
+        const int mine = threadIdx.x & 7;
+        tm = -INFINITY;
         tl = 0.f;
 #pragma unroll
         for (int d = 0; d < kPer; ++d) v[d] = 0.f;
-#pragma unroll 4
-        for (int c = -1; c < c1 - c0; ++c) {
-          const float *p = c < 0 ? p0 : p1 + static_cast<int64_t>(c) * 2 * Z::kPartFloats;
-          const float f = exp2_approx((__ldcg(p + kRowsTile * D + r) - use) * A.scale_log2);
-          tl = fmaf(__ldcg(p + kRowsTile * (D + 1) + r), f, tl);
+#pragma unroll 2
+        for (int k0 = 0; k0 < parts; k0 += 8) {
+          const float *own = part_at(min(k0 + mine, parts - 1)) + kRowsTile * D + r;
+          float pm = __ldcg(own), pl = __ldcg(own + kRowsTile);
+          float4 y[8][kPer / 4];
 #pragma unroll
-          for (int d = 0; d < kPer; d += 4) {
-            const float4 y = __ldcg(reinterpret_cast<const float4 *>(p + r * D + d0 + d));
-            v[d] = fmaf(y.x, f, v[d]);
-            v[d + 1] = fmaf(y.y, f, v[d + 1]);
-            v[d + 2] = fmaf(y.z, f, v[d + 2]);
-            v[d + 3] = fmaf(y.w, f, v[d + 3]);
+          for (int x = 0; x < 8; ++x)
+#pragma unroll
+            for (int d = 0; d < kPer / 4; ++d)
+              y[x][d] = k0 + x < parts ? __ldcg(reinterpret_cast<const float4 *>(part_at(k0 + x) + r * D + d0) + d)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+          if (k0 + mine >= parts) pm = -INFINITY;
+          float top = pm;
+#pragma unroll
+          for (int x = 1; x < 8; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          top = fmaxf(top, tm);
+          const float use = top == -INFINITY ? 0.f : top;
+          const float old = exp2_approx((tm - use) * A.scale_log2), f = exp2_approx((pm - use) * A.scale_log2);
+          tm = top;
+          float sum = f * pl;
+          if (k0 + mine >= parts) sum = 0.f;
+#pragma unroll
+          for (int x = 1; x < 8; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+          tl = fmaf(tl, old, sum);
+#pragma unroll
+          for (int d = 0; d < kPer; ++d) v[d] *= old;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float g = __shfl_sync(0xffffffffu, f, (lane & 24) + x);
+#pragma unroll
+            for (int d = 0; d < kPer / 4; ++d) {
+              v[4 * d] = fmaf(y[x][d].x, g, v[4 * d]);
+              v[4 * d + 1] = fmaf(y[x][d].y, g, v[4 * d + 1]);
+              v[4 * d + 2] = fmaf(y[x][d].z, g, v[4 * d + 2]);
+              v[4 * d + 3] = fmaf(y[x][d].w, g, v[4 * d + 3]);
+            }
           }
         }
       }

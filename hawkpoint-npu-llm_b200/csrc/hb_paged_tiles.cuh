@@ -31,6 +31,7 @@ namespace paged {
 
 constexpr int kTilesTile = 256, kTilesHalf = 128, kTilesBlock = 128;
 constexpr int kTilesExtra = 2;   // a tile's start and end, in blocks
+constexpr int kTilesLeast = 3;   // units a piece has at least
 constexpr int kTurnAt = 5;   // of eight parts of its exponentials, those a half has added up when it passes its turn on
 constexpr int kTilesThreads = 384;
 // Registers a thread after the split: 256 softmax threads x 216 + 128 others x
@@ -251,9 +252,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     fence_mbar_init();
   }
   fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group > A.few; });
-  const int64_t total = line.prefix[A.batch.entries];
-  const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + least - 1) / least));
-  if (static_cast<int>(blockIdx.x) >= pieces) return;
+  const Cut cut(line.prefix[A.batch.entries], gridDim.x, least);
+  if (static_cast<int>(blockIdx.x) >= cut.pieces) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // as at the end
+    return;
+  }
   if (warp == 0) t_alloc(&s_tmem, 512);
   t_before();
   __syncthreads();
@@ -261,8 +264,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   // 512 columns are all of them: the allocation starts at column 0
 
   Walk w;
-  w.u = piece_begin(total, pieces, blockIdx.x);
-  w.end = piece_begin(total, pieces, blockIdx.x + 1);
+  w.u = cut.begin(blockIdx.x);
+  w.end = cut.begin(blockIdx.x + 1);
   bool more = w.start(A.pool, A.batch, S, line);
   auto halves = [&]() { return w.e.n * S.group - w.t * kTilesTile > kTilesHalf ? 2 : 1; };
 
@@ -481,8 +484,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         info.opens = w.opens();
         info.hole = hole;
         if (!w.whole()) {
-          info.c0 = piece_of(total, pieces, w.tile_u + S.extra);
-          info.c1 = piece_of(total, pieces, w.tile_u + w.units - 1);
+          info.c0 = cut.of(w.tile_u + S.extra);
+          info.c1 = cut.of(w.tile_u + w.units - 1);
         }
       }
       cp_async_wait_all();
@@ -651,20 +654,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         }
         __stcg(part + 128 * D + r, m);
         __stcg(part + 128 * (D + 1) + r, l);
-        __threadfence();
         if (!half_sync()) break;   // the half's part is written
         c0 = info.c0;
         c1 = info.c1;
         if (r == 0) {
-          const int before = atomicAdd(&A.arrived[2 * c0 + h], 1);
-          s_last[h] = before == c1 - c0;
+          s_last[h] = arrive_acq_rel(&A.arrived[2 * c0 + h]) == c1 - c0;
           if (s_last[h]) A.arrived[2 * c0 + h] = 0;
         }
         if (!half_sync()) break;
         write = write && s_last[h] != 0;
         if (!half_sync()) break;   // s_last is read
         if (write) {
-          __threadfence();
           const float *p = A.parts + h * Z::kPartFloats + 128 * D + r;
           m = -INFINITY;
           for (int k = c0; k <= c1; ++k) m = fmaxf(m, __ldcg(p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo));
@@ -749,6 +749,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   __syncthreads();
   t_after();
   if (warp == 0) t_dealloc(s_tmem, 512);
+  // launched beside the rows kernel of the same call, this one is not done
+  // before that one
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace paged
