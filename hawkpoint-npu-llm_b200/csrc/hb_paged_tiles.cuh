@@ -30,7 +30,7 @@ namespace hb {
 namespace paged {
 
 constexpr int kTilesTile = 256, kTilesHalf = 128, kTilesBlock = 128;
-constexpr int kTilesExtra = 2;   // a tile's start and end, in blocks
+constexpr int kTilesExtra = 1;   // a tile's start and end, in blocks
 constexpr int kTilesLeast = 3;   // units a piece has at least
 constexpr int kTurnAt = 5;   // of eight parts of its exponentials, those a half has added up when it passes its turn on
 constexpr int kTilesThreads = 384;
@@ -449,19 +449,41 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       }
       const int packed = w.e.n * S.group, base = w.t * kTilesTile + h * kTilesHalf;
       uint8_t *dst = smem + (buf * 2 + h) * Z::kOperand;
-      // a lane 16 bytes; D / 8 lanes a row
-      const int c = lane % (D / 8);
-      for (int r = lane / (D / 8); r < kTilesHalf; r += 256 / D) {
-        uint8_t *to = dst + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        const int row = base + r, i = S.row_of(row), g = row - i * S.group;
-        const uint16_t *q = static_cast<const uint16_t *>(A.q) + (w.e.row0 + i) * A.q_row +
-                            (w.head * S.group + g) * A.q_head + c * 8;
-        if (row >= packed)
-          *reinterpret_cast<uint4 *>(to) = make_uint4(0, 0, 0, 0);
-        else if (A.q_vec)
-          cp_async16(to, q);
-        else
-          *reinterpret_cast<uint4 *>(to) = load8<false>(q);
+      // a lane 16 bytes, D / 8 lanes a row; each lane finds four of the rows
+      uint64_t rows[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int row = base + 32 * x + lane, i = S.row_of(row), g = row - i * S.group;
+        rows[x] = row < packed ? reinterpret_cast<uint64_t>(static_cast<const uint16_t *>(A.q) + (w.e.row0 + i) * A.q_row +
+                                                            (w.head * S.group + g) * A.q_head)
+                               : 0;
+      }
+      constexpr int kPer = D / 8, kRows = 32 / kPer;   // 16-byte parts of a row; rows a step
+      const int c = lane % kPer, sub = lane / kPer;
+      uint8_t *to = dst + (c >> 3) * 16384;
+      auto copy = [&](int x, int y, bool vec) {
+        const int rr = y * kRows + sub, r = 32 * x + rr;
+        const uint64_t from = __shfl_sync(0xffffffffu, rows[x], rr);
+        uint8_t *at = to + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        if (vec) {   // rows that are not there: no bytes read, zeros written
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(at)),
+                       "l"(from != 0 ? from + c * 16 : reinterpret_cast<uint64_t>(A.q)), "r"(from != 0 ? 16 : 0)
+                       : "memory");
+        } else {
+          *reinterpret_cast<uint4 *>(at) =
+              from != 0 ? load8<false>(reinterpret_cast<const uint16_t *>(from) + c * 8) : make_uint4(0, 0, 0, 0);
+        }
+      };
+      if (A.q_vec) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll 8
+          for (int y = 0; y < kPer; ++y) copy(x, y, true);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll 1
+          for (int y = 0; y < kPer; ++y) copy(x, y, false);
       }
       cp_async_commit();
       const int first = w.first(), count = w.count(S);
@@ -667,11 +689,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         if (write) {
           const float *p = A.parts + h * Z::kPartFloats + 128 * D + r;
           m = -INFINITY;
-          for (int k = c0; k <= c1; ++k) m = fmaxf(m, __ldcg(p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo));
           l = 0.f;
+#pragma unroll 4
           for (int k = c0; k <= c1; ++k) {
             const float *pk = p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo;
-            l = fmaf(__ldcg(pk + 128), exp2_approx((__ldcg(pk) - (m == -INFINITY ? 0.f : m)) * c), l);
+            const float pm = __ldcg(pk), pl = __ldcg(pk + 128), nm = fmaxf(m, pm), use = nm == -INFINITY ? 0.f : nm;
+            l = l * exp2_approx((m - use) * c) + pl * exp2_approx((pm - use) * c);
+            m = nm;
           }
         }
       }
@@ -683,45 +707,49 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       T *out = static_cast<T *>(A.out) + orow * A.o_row + qh * A.o_head;
       uint64_t wrong = 0;   // NaN as soon as a value is not finite
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x) {
-        float o[32];
+      for (int x = 0; x < D / 64; ++x) {   // 64 dims at a time
+        float o[64];
         if (whole) {
-          t_ld32(t_o + x * 32, o);
+          t_ld32(t_o + x * 64, o);
+          t_ld32(t_o + x * 64 + 32, o + 32);
           t_ld_wait();
         } else if (write) {
           const float *p = A.parts + h * Z::kPartFloats;
 #pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = 0.f;
+          for (int y = 0; y < 64; ++y) o[y] = 0.f;
+#pragma unroll 2
           for (int k = c0; k <= c1; ++k) {
             const float *pk = p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo;
             const float f = exp2_approx((__ldcg(pk + 128 * D + r) - (m == -INFINITY ? 0.f : m)) * c);
+            float4 v[16];
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-              const float4 v = __ldcg(reinterpret_cast<const float4 *>(pk) + (x * 8 + y) * 128 + r);
-              o[4 * y] = fmaf(v.x, f, o[4 * y]);
-              o[4 * y + 1] = fmaf(v.y, f, o[4 * y + 1]);
-              o[4 * y + 2] = fmaf(v.z, f, o[4 * y + 2]);
-              o[4 * y + 3] = fmaf(v.w, f, o[4 * y + 3]);
+            for (int y = 0; y < 16; ++y) v[y] = __ldcg(reinterpret_cast<const float4 *>(pk) + (x * 16 + y) * 128 + r);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+              o[4 * y] = fmaf(v[y].x, f, o[4 * y]);
+              o[4 * y + 1] = fmaf(v[y].y, f, o[4 * y + 1]);
+              o[4 * y + 2] = fmaf(v[y].z, f, o[4 * y + 2]);
+              o[4 * y + 3] = fmaf(v[y].w, f, o[4 * y + 3]);
             }
           }
         }
         if (write) {
-          uint32_t u[16];
+          uint32_t u[32];
 #pragma unroll
-          for (int y = 0; y < 16; ++y) {
+          for (int y = 0; y < 32; ++y) {
             const uint64_t v = f2_mul(f2(o[2 * y], o[2 * y + 1]), f2(inv, inv));
             wrong = f2_fma(v, 0, wrong);
             float a, b;
             f2_split(v, a, b);
             u[y] = E::pack(a, b);
           }
-          uint16_t *dst = reinterpret_cast<uint16_t *>(out) + x * 32;
+          uint16_t *dst = reinterpret_cast<uint16_t *>(out) + x * 64;
           if (A.o_wide) {
 #pragma unroll
-            for (int y = 0; y < 2; ++y) store32(dst + y * 16, u + y * 8);
+            for (int y = 0; y < 4; ++y) store32(dst + y * 16, u + y * 8);
           } else {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
+            for (int y = 0; y < 8; ++y) {
               const uint4 v = make_uint4(u[4 * y], u[4 * y + 1], u[4 * y + 2], u[4 * y + 3]);
               if (A.o_vec) store8<true>(dst + y * 8, v); else store8<false>(dst + y * 8, v);
             }
