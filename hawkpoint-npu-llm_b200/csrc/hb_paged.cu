@@ -13,6 +13,8 @@ namespace pg = hb::paged;
 namespace {
 
 constexpr int kMaxDevices = 64;
+constexpr int kAppendMost = pg::kAppendRows;
+constexpr int kAppendBlocks = 8;
 
 // What a device's calls need to know, looked up on the first of them.
 struct DeviceInfo {
@@ -226,10 +228,14 @@ cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) 
 
 template <int D, class T>
 cudaError_t launch_append(const pg::Append &A, bool vec, int grid, cudaStream_t st) {
+  // whole rows a block: as many as fit, a row's part a thread
+  const int parts = (A.q_heads + 2 * A.pool.kv_heads) * (D / 16);
+  const int threads = parts >= pg::kAppendThreads ? pg::kAppendThreads
+                                                  : (pg::kAppendThreads / parts * parts + 31) / 32 * 32;
   if (vec)
-    pg::paged_append_kernel<D, T, true><<<grid, pg::kAppendThreads, 0, st>>>(A);
+    pg::paged_append_kernel<D, T, true><<<grid, threads, 0, st>>>(A);
   else
-    pg::paged_append_kernel<D, T, false><<<grid, pg::kAppendThreads, 0, st>>>(A);
+    pg::paged_append_kernel<D, T, false><<<grid, threads, 0, st>>>(A);
   return cudaGetLastError();
 }
 
@@ -357,7 +363,7 @@ int hb_paged_append(const hb_page_pool *pool, int layer, const hb_paged_rows *ro
   A.rope_positions = n->rope_positions;
   A.q_heads = n->q_heads;
   // few rows: a block each; many: enough blocks for every multiprocessor
-  A.block_rows = std::max(1, std::min(pg::kAppendRows, rows->rows / (4 * sms)));
+  A.block_rows = std::max(1, std::min(kAppendMost, (rows->rows + kAppendBlocks * sms - 1) / (kAppendBlocks * sms)));
   const bool vec = vec_ok(n->qkv_dev, n->qkv_row_stride, 0) && vec_ok(n->q_dev, n->q_row_stride, n->q_head_stride);
   const int grid = (rows->rows + A.block_rows - 1) / A.block_rows;
   const bool bf = pool->element == HB_ELEM_BF16;

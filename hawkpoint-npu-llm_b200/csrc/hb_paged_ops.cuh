@@ -35,7 +35,7 @@ struct Append {
   int rope_positions, q_heads;
   int block_rows;                // rows a block
 };
-constexpr int kAppendThreads = 256, kAppendRows = 16;
+constexpr int kAppendThreads = 256, kAppendRows = 64;   // the most of a block
 
 template <class T>
 __device__ __forceinline__ void rope8(const uint4 &x0, const uint4 &x1, const float *c, const float *s, uint4 &lo,
@@ -59,66 +59,94 @@ template <int D, class T, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ Append A) {
   __shared__ int s_pos[kAppendRows], s_page[kAppendRows];
   const int row0 = blockIdx.x * A.block_rows, rows = min(A.block_rows, A.batch.rows - row0);
-  if (static_cast<int>(threadIdx.x) < rows) {
-    const int row = row0 + threadIdx.x;
-    int lo = 0, hi = A.batch.entries;   // the last entry that starts at or before the row
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(A.batch.row_start + mid) <= row) lo = mid; else hi = mid;
+  // a thread keeps its part of a head (8 dims of either half) and takes every
+  // `step`-th row, the next one's reads ahead
+  constexpr int kPer = D / 16;
+  const int kvh = A.pool.kv_heads, parts = (A.q_heads + 2 * kvh) * kPer;
+  const int step = max(1, static_cast<int>(blockDim.x) / parts);
+  const int lanes = step * parts;   // threads at work; a row with more parts than threads takes turns
+  const uint16_t *qkv = static_cast<const uint16_t *>(A.qkv) + row0 * A.qkv_row;
+  int x = threadIdx.x, r = x / parts;
+  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+  const auto part_of = [&](int i) { return i % parts / kPer * D + i % parts % kPer * 8; };
+  if (x < lanes && r < rows) {   // does not wait for the positions
+    lo = load8<VEC>(qkv + r * A.qkv_row + part_of(x));
+    hi = load8<VEC>(qkv + r * A.qkv_row + part_of(x) + D / 2);
+  }
+  if (threadIdx.x < 32) {
+    // the entry of the block's first row by 32-way search, a lane's own from there
+    const int lane = threadIdx.x;
+    int first = 0, n = A.batch.entries;
+    while (n > 1) {
+      const int stride = (n + 31) / 32, i = first + lane * stride;
+      const bool in = lane * stride < n && __ldg(A.batch.row_start + i) <= row0;
+      const int k = max(0, 31 - __clz(__ballot_sync(0xffffffffu, in)));   // the last that starts at or before the row
+      first += k * stride;
+      n = min(stride, n - k * stride);
     }
-    const Entry e = entry_of(A.pool, A.batch, lo);
-    int pos = e.length - e.n + row - e.row0, pg = -1, bad = 0;
-    if (row < e.row0 || row >= e.row0 + e.n || e.slot < 0 || pos < 0) {
-      pos = -1;            // no entry's row, or before its sequence: nothing to append, no position to turn to
-    } else {
-      pg = page_of(A.pool, e.slot, pos >> 6);
-      if (pg < 0) bad = HB_PAGED_UNMAPPED;
-      if (pos >= A.rope_positions) {
-        bad |= HB_PAGED_BAD_INDEX;
-        pos = pg = -1;
+    for (int i = lane; i < rows; i += 32) {
+      const int row = row0 + i;
+      int b = first;
+      while (b + 1 < A.batch.entries && __ldg(A.batch.row_start + b + 1) <= row) ++b;
+      const Entry e = entry_of(A.pool, A.batch, b);
+      int pos = e.length - e.n + row - e.row0, pg = -1, bad = 0;
+      if (row < e.row0 || row >= e.row0 + e.n || e.slot < 0 || pos < 0) {
+        pos = -1;            // no entry's row, or before its sequence: nothing to append, no position to turn to
+      } else {
+        pg = page_of(A.pool, e.slot, pos >> 6);
+        if (pg < 0) bad = HB_PAGED_UNMAPPED;
+        if (pos >= A.rope_positions) {
+          bad |= HB_PAGED_BAD_INDEX;
+          pos = pg = -1;
+        }
       }
+      if (bad) atomicOr(&A.pool.control->status, bad);
+      // a reserve that ran out of pages left lengths and pages as they were: these are not this row's places
+      if (ld_volatile_int(&A.pool.control->status) & HB_PAGED_EXHAUSTED) pg = -1;
+      s_pos[i] = pos;
+      s_page[i] = pg;
     }
-    if (bad) atomicOr(&A.pool.control->status, bad);
-    // a reserve that ran out of pages left lengths and pages as they were: these are not this row's places
-    if (ld_volatile_int(&A.pool.control->status) & HB_PAGED_EXHAUSTED) pg = -1;
-    s_pos[threadIdx.x] = pos;
-    s_page[threadIdx.x] = pg;
   }
   __syncthreads();
-  constexpr int kPer = D / 16;   // threads a head
-  const int kvh = A.pool.kv_heads, heads = A.q_heads + 2 * kvh;
-  for (int x = threadIdx.x; x < rows * heads * kPer; x += kAppendThreads) {
-    const int c = x % kPer, y = x / kPer, head = y % heads, r = y / heads, row = row0 + r;
-    const int pos = s_pos[r], pg = s_page[r];
-    const uint16_t *src = static_cast<const uint16_t *>(A.qkv) + row * A.qkv_row + head * D + c * 8;
+  for (; x < lanes; x += blockDim.x, r = x / parts) {
+    const int part = x % parts, c = part % kPer, head = part / kPer;
     const bool is_v = head >= A.q_heads + kvh, is_q = head < A.q_heads;
-    if (!is_q && pg < 0) continue;
-    uint4 lo = load8<VEC>(src), hi = load8<VEC>(src + D / 2);
-    if (!is_v) {
-      if (pos < 0) {
-        lo = hi = make_uint4(0, 0, 0, 0);
-      } else {
-        float cs[8], sn[8];
-        const float4 *cp = reinterpret_cast<const float4 *>(A.cos + static_cast<int64_t>(pos) * (D / 2) + c * 8);
-        const float4 *sp = reinterpret_cast<const float4 *>(A.sin + static_cast<int64_t>(pos) * (D / 2) + c * 8);
-        const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
-        cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w; cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
-        sn[0] = s0.x; sn[1] = s0.y; sn[2] = s0.z; sn[3] = s0.w; sn[4] = s1.x; sn[5] = s1.y; sn[6] = s1.z; sn[7] = s1.w;
-        rope8<T>(lo, hi, cs, sn, lo, hi);
-      }
+    const int h = is_v ? head - A.q_heads - kvh : head - A.q_heads;
+    uint8_t *kv = A.pool.pages + A.layer_off + h * A.head_bytes + (is_v ? D / 64 * kBlockBytes : 0);
+    uint16_t *q = static_cast<uint16_t *>(A.q) + row0 * A.q_row + head * A.q_head + c * 8;
+    const uint16_t *src = qkv + part_of(x);
+    const int d0 = c * 8, d1 = D / 2 + c * 8;
+    if (x != static_cast<int>(threadIdx.x) && r < rows) {
+      lo = load8<VEC>(src + r * A.qkv_row);
+      hi = load8<VEC>(src + r * A.qkv_row + D / 2);
     }
-    if (is_q) {
-      uint16_t *dst = static_cast<uint16_t *>(A.q) + row * A.q_row + head * A.q_head + c * 8;
-      store8<VEC>(dst, lo);
-      store8<VEC>(dst + D / 2, hi);
-    } else {
-      const int h = is_v ? head - A.q_heads - kvh : head - A.q_heads;
-      uint8_t *dst = A.pool.pages + static_cast<int64_t>(pg) * A.pool.page_stride + A.layer_off + h * A.head_bytes +
-                     (is_v ? D / 64 * kBlockBytes : 0);
-      // the low half's dims 8 c .. and the high half's D / 2 + 8 c ..
-      const int d0 = c * 8, d1 = D / 2 + c * 8;
-      *reinterpret_cast<uint4 *>(dst + (d0 >> 6) * kBlockBytes + kv_off(pos & 63, (d0 & 63) >> 3)) = lo;
-      *reinterpret_cast<uint4 *>(dst + (d1 >> 6) * kBlockBytes + kv_off(pos & 63, (d1 & 63) >> 3)) = hi;
+    for (; r < rows; r += step) {
+      const int pos = s_pos[r], pg = s_page[r];
+      uint4 a = lo, b = hi;
+      if (r + step < rows) {
+        lo = load8<VEC>(src + (r + step) * A.qkv_row);
+        hi = load8<VEC>(src + (r + step) * A.qkv_row + D / 2);
+      }
+      if (!is_v) {
+        if (pos >= 0) {
+          const int64_t off = static_cast<int64_t>(pos) * (D / 2) + c * 8;
+          const float4 c0 = __ldg(reinterpret_cast<const float4 *>(A.cos + off)), c1 = __ldg(reinterpret_cast<const float4 *>(A.cos + off) + 1);
+          const float4 s0 = __ldg(reinterpret_cast<const float4 *>(A.sin + off)), s1 = __ldg(reinterpret_cast<const float4 *>(A.sin + off) + 1);
+          const float cv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+          const float sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+          rope8<T>(a, b, cv, sv, a, b);
+        } else {
+          a = b = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (is_q) {
+        store8<VEC>(q + r * A.q_row, a);
+        store8<VEC>(q + r * A.q_row + D / 2, b);
+      } else if (pg >= 0) {
+        uint8_t *dst = kv + pg * A.pool.page_stride;
+        *reinterpret_cast<uint4 *>(dst + (d0 >> 6) * kBlockBytes + kv_off(pos & 63, (d0 & 63) >> 3)) = a;
+        *reinterpret_cast<uint4 *>(dst + (d1 >> 6) * kBlockBytes + kv_off(pos & 63, (d1 & 63) >> 3)) = b;
+      }
     }
   }
 }
