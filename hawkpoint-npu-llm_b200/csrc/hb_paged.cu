@@ -408,7 +408,10 @@ int hb_pages_fork(const hb_page_pool *pool, int n, const int32_t *src_dev, const
   const pg::Pool v = pool_view(*pool);
   pg::fork_kernel<<<1, pg::kBookThreads, 0, st>>>(v, x, src_dev, dst_dev, counts_dev, n);
   HB_CUDA(nullptr, cudaGetLastError());
-  return launch_copy(*pool, pool->pages_dev, pool->n_pages, x.from, x.to, x.held, &v.control->copies, 0, nullptr, 4 * sms, st);
+  // a warp an 8 KB block to copy, as far as the GPU holds them at once
+  const int64_t most = (static_cast<int64_t>(n) * (layer_bytes(*pool) * pool->layers / pg::kBlockBytes) + 7) / 8;
+  return launch_copy(*pool, pool->pages_dev, pool->n_pages, x.from, x.to, x.held, &v.control->copies, 0, nullptr,
+                     static_cast<int>(std::min<int64_t>(most, 8 * sms)), st);
 }
 
 int hb_pages_free(const hb_page_pool *pool, int n, const int32_t *slots_dev, void *stream) {

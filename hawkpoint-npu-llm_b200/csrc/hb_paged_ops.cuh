@@ -315,6 +315,9 @@ __global__ void __launch_bounds__(kBookThreads) reserve_kernel(Pool P, Scratch X
   }
 }
 
+// The rows of a call that fit, being made in shared memory.
+constexpr int kStageInts = 8192;
+
 // hb_pages_fork: dst[b] becomes the first counts[b] positions of src[b], all
 // sources as they were before the call (so a permutation of slots, as a beam
 // search's, is one call).  Whole pages are shared; the positions of a partial
@@ -322,54 +325,50 @@ __global__ void __launch_bounds__(kBookThreads) reserve_kernel(Pool P, Scratch X
 __global__ void __launch_bounds__(kBookThreads) fork_kernel(Pool P, Scratch X, const int *src, const int *dst,
                                                             const int *counts, int n) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the copy kernel's blocks may take their places
-  __shared__ int s_sums[32], s_bad;
+  __shared__ int s_sums[32], s_bad, s_stage[kStageInts];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     s_bad = 0;
     P.control->copies = 0;
   }
+  // at most a page an entry: looked for while the entries are read
+  const int free = lowest_free(P.refs, P.n_pages, n, X.fresh, s_sums);
   __syncthreads();
   for (int b = threadIdx.x; b < n; b += kBookThreads) {
     const int from = src[b], to = dst[b], count = counts[b];
     int need = 0;
-    if (from < 0 || from >= P.n_slots || to < 0 || to >= P.n_slots || count < 0 || count > P.lengths[from] ||
-        count > P.width * kPage || atomicExch(&X.mark[to], 1) != 0) {
+    if (from < 0 || from >= P.n_slots || to < 0 || to >= P.n_slots || count < 0 || count > P.width * kPage) {
       atomicOr(&s_bad, HB_PAGED_BAD_INDEX);
     } else {
-      need = count % kPage != 0 && page_of(P, from, count / kPage) >= 0 ? 1 : 0;
+      const int length = P.lengths[from], page = page_of(P, from, count / kPage);
+      if (atomicExch(&X.mark[to], 1) != 0 || count > length) atomicOr(&s_bad, HB_PAGED_BAD_INDEX);
+      need = count % kPage != 0 && page >= 0 ? 1 : 0;
     }
     X.need[b] = need;
   }
   __syncthreads();
   const int total = scan_needs(X.need, X.off, n, s_sums);
-  if (s_bad == 0 && total > 0 && (total > P.n_pages || lowest_free(P.refs, P.n_pages, total, X.fresh, s_sums) < total)) {
-    __syncthreads();
-    if (threadIdx.x == 0) s_bad = HB_PAGED_EXHAUSTED;
-  }
   for (int b = threadIdx.x; b < n; b += kBookThreads)
     if (dst[b] >= 0 && dst[b] < P.n_slots) X.mark[dst[b]] = 0;
-  __syncthreads();
-  if (s_bad) {
-    if (threadIdx.x == 0) atomicOr(&P.control->status, s_bad);
+  if (s_bad || total > free) {   // all or nothing
+    if (threadIdx.x == 0) atomicOr(&P.control->status, s_bad ? s_bad : HB_PAGED_EXHAUSTED);
     return;
   }
+  __syncthreads();
   // the new rows beside the old ones, and the counts: what the sources share,
   // what the destinations give up (additions, so in any order)
+  int *stage = static_cast<int64_t>(n) * P.width <= kStageInts ? s_stage : X.stage;
   for (int b = warp; b < n; b += 32) {
-    const int from = src[b], to = dst[b], count = counts[b], whole = count / kPage;
+    const int from = src[b], to = dst[b], count = counts[b], whole = count / kPage, need = X.need[b];
+    const int fresh = need ? X.fresh[X.off[b]] : -1;
     for (int i = lane; i < P.width; i += 32) {
       const int gone = page_of(P, to, i);
       int now = i <= whole ? page_of(P, from, i) : -1;
       if (i == whole) {
-        if (X.need[b]) {
-          const int fresh = X.fresh[X.off[b]];
-          push_copy(P, X, now, fresh, count % kPage);
-          now = fresh;
-        } else {
-          now = -1;
-        }
+        if (need) push_copy(P, X, now, fresh, count % kPage);
+        now = fresh;
       }
-      X.stage[static_cast<int64_t>(to) * P.width + i] = now;
+      stage[static_cast<int64_t>(b) * P.width + i] = now;
       if (now >= 0) atomicAdd(&P.refs[now], 1);
       if (gone >= 0) atomicSub(&P.refs[gone], 1);
     }
@@ -377,7 +376,7 @@ __global__ void __launch_bounds__(kBookThreads) fork_kernel(Pool P, Scratch X, c
   __syncthreads();
   for (int b = warp; b < n; b += 32) {
     const int64_t row = static_cast<int64_t>(dst[b]) * P.width;
-    for (int i = lane; i < P.width; i += 32) P.table[row + i] = X.stage[row + i];
+    for (int i = lane; i < P.width; i += 32) P.table[row + i] = stage[static_cast<int64_t>(b) * P.width + i];
     if (lane == 0) P.lengths[dst[b]] = counts[b];
   }
 }
