@@ -112,7 +112,7 @@ __device__ __forceinline__ bool store_row(const Attend &A, const Entry &e, int h
 }
 
 template <int D, class T>
-__global__ void __launch_bounds__(kRowsThreads) paged_rows_kernel(const __grid_constant__ Attend A, int least) {
+__global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kernel(const __grid_constant__ Attend A, int least) {
   using E = Elem<T>;
   using Z = RowsSize<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
