@@ -122,6 +122,7 @@ template <class Take>
 __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const Shape &S, const Line &line,
                                           const Take &take) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll 1
   for (int b0 = warp * 32; b0 < B.entries; b0 += blockDim.x) {
     const int b = b0 + lane;
     Entry e{0, 0, 0, -1};
@@ -129,11 +130,13 @@ __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const S
     const int tiles = b < B.entries && take(e) ? tiles_of(S, e) : 0;
     int u = 0;
     if (tiles <= 4)
+#pragma unroll 1
       for (int t = 0; t < tiles; ++t) u += tile_units(S, e, t);
     for (unsigned many = __ballot_sync(0xffffffffu, tiles > 4); many; many &= many - 1) {
       const int x = __ffs(many) - 1, n = __shfl_sync(0xffffffffu, tiles, x);
       const Entry y{0, __shfl_sync(0xffffffffu, e.n, x), __shfl_sync(0xffffffffu, e.length, x), 0};
       int v = 0;
+#pragma unroll 1
       for (int t = lane; t < n; t += 32) v += tile_units(S, y, t);
       v = __reduce_add_sync(0xffffffffu, v);
       if (lane == x) u = v;
@@ -143,6 +146,7 @@ __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const S
   __syncthreads();
   if (warp == 0) {
     int base = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < B.entries; b0 += 32) {
       const int b = b0 + lane;
       int v = b < B.entries ? line.prefix[b + 1] : 0;

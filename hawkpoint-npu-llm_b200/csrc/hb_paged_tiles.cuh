@@ -314,16 +314,23 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     };
     for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
       const int first = w.first(), count = w.count(S);
-      int mine = -1, v0 = -1, v1 = -1;
-      for (int j = 0; j < count && ok; ++j) {
-        if ((j & 15) == 0) mine = page_of(A.pool, w.e.slot, 2 * (first + j) + lane);
-        const int k0 = __shfl_sync(0xffffffffu, mine, 2 * (j & 15)), k1 = __shfl_sync(0xffffffffu, mine, 2 * (j & 15) + 1);
-        load(false, first + j, k0, k1);
-        if (j > 0 && ok) load(true, first + j - 1, v0, v1);
-        v0 = k0;
-        v1 = k1;
+      int mine = -1, k0 = -1, k1 = -1, v0 = -1, v1 = -1;
+      // K(0), then K(j), V(j - 1) in turn, at last V(count - 1).  One place for
+      // all loads: the warps' loops share the instruction cache.
+#pragma unroll 1
+      for (int x = 0; x < 2 * count && ok; ++x) {
+        const bool last = x == 2 * count - 1, is_v = last || (x != 0 && (x & 1) == 0);
+        int block = last ? count - 1 : (x >> 1) - 1, p0 = last ? k0 : v0, p1 = last ? k1 : v1;
+        if (!is_v) {
+          block = (x + 1) >> 1;
+          if ((block & 15) == 0) mine = page_of(A.pool, w.e.slot, 2 * (first + block) + lane);
+          v0 = k0;
+          v1 = k1;
+          p0 = k0 = __shfl_sync(0xffffffffu, mine, 2 * (block & 15));
+          p1 = k1 = __shfl_sync(0xffffffffu, mine, 2 * (block & 15) + 1);
+        }
+        load(is_v, first + block, p0, p1);
       }
-      if (ok) load(true, first + count - 1, v0, v1);
     }
     for (int i = max(0, it - Z::kStages); i < it; ++i)   // nothing in flight when the block ends
       mbar_wait_quiet(&bars.full[i % Z::kStages], static_cast<uint32_t>(i / Z::kStages) & 1u, A.limit_ns);
@@ -335,7 +342,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     const uint32_t q_lo = swizzled_lo(smem_u32(smem), 16), k_lo = swizzled_lo(smem_u32(ring), 16),
                    v_lo = swizzled_lo(smem_u32(ring), 16384);
     uint32_t it = 0;                // ring stages consumed
-    uint32_t n_q0 = 0, n_q1 = 0, n_s0 = 0, n_s1 = 0;   // tiles and steps of either half so far
+    uint32_t n_q0 = 0, n_q1 = 0, n_s[2] = {0, 0};   // tiles and steps of either half so far
     bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t phase) {
       ok = __all_sync(0xffffffffu, ok && t_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
@@ -381,49 +388,31 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         wait(&bars.q_full[1][buf1], n_q1 / Z::kQ);
         ++n_q1;
       }
-      if (!wait_ring(it)) break;
-      mma_s(0, buf0, it);
-      if (two) mma_s(1, buf1, it);
-      commit(&bars.empty[stage(it)]);
-      for (uint32_t j = 0; j < count; ++j) {
-        const bool next = j + 1 < count;
-        const uint32_t ik = it + 2 * j + 1, iv = next ? ik + 1 : ik;
+      // steps -1 (the first S alone), 0 .. count - 1: the next step's S, this
+      // one's O; one place for either, the warps' loops share the instruction cache
+#pragma unroll 1
+      for (int j = -1; ok && j < static_cast<int>(count); ++j) {
+        const bool next = j + 1 < static_cast<int>(count);
+        const uint32_t ik = it + (j < 0 ? 0 : 2 * j + 1), iv = next ? ik + 1 : ik;
         if (!next) {   // every S of the tile is issued
           commit(&bars.q_empty[0][buf0]);
           if (two) commit(&bars.q_empty[1][buf1]);
         }
         if (next && !wait_ring(ik)) break;
-        if constexpr (Z::kEarly) {
-          if (next) {
-            if (!wait(&bars.s_read[0], n_s0)) break;
-            mma_s(0, buf0, ik);
-            if (two) {
-              if (!wait(&bars.s_read[1], n_s1)) break;
-              mma_s(1, buf1, ik);
-            }
-            commit(&bars.empty[stage(ik)]);
-          }
-          if (!wait_ring(iv)) break;
-          if (!wait(&bars.p_full[0], n_s0++)) break;
-          mma_o(0, iv, j != 0);
-          if (two) {
-            if (!wait(&bars.p_full[1], n_s1++)) break;
-            mma_o(1, iv, j != 0);
-          }
-          commit(&bars.empty[stage(iv)]);
-        } else {
-          if (!wait_ring(iv)) break;
-          if (!wait(&bars.p_full[0], n_s0++)) break;
-          mma_o(0, iv, j != 0);
-          if (next) mma_s(0, buf0, ik);   // over the P just used: MMAs run in order
-          if (two) {
-            if (!wait(&bars.p_full[1], n_s1++)) break;
-            mma_o(1, iv, j != 0);
-            if (next) mma_s(1, buf1, ik);
-          }
-          if (next) commit(&bars.empty[stage(ik)]);
-          commit(&bars.empty[stage(iv)]);
+        if (Z::kEarly && next) {
+#pragma unroll 1
+          for (int h = 0; h < (two ? 2 : 1); ++h)
+            if (j < 0 || wait(&bars.s_read[h], n_s[h])) mma_s(h, h ? buf1 : buf0, ik);
+          commit(&bars.empty[stage(ik)]);
         }
+        if (j >= 0 && !wait_ring(iv)) break;
+#pragma unroll 1
+        for (int h = 0; h < (two ? 2 : 1); ++h) {
+          if (j >= 0 && wait(&bars.p_full[h], n_s[h]++)) mma_o(h, iv, j != 0);
+          if (!Z::kEarly && next && ok) mma_s(h, h ? buf1 : buf0, ik);   // over the P just used: MMAs run in order
+        }
+        if (!Z::kEarly && next) commit(&bars.empty[stage(ik)]);
+        if (j >= 0) commit(&bars.empty[stage(iv)]);
       }
       it += 2 * count;
     }
@@ -449,21 +438,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       }
       const int packed = w.e.n * S.group, base = w.t * kTilesTile + h * kTilesHalf;
       uint8_t *dst = smem + (buf * 2 + h) * Z::kOperand;
-      // a lane 16 bytes, D / 8 lanes a row; each lane finds four of the rows
-      uint64_t rows[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
+      // a lane 16 bytes, D / 8 lanes a row; each lane finds one of 32 rows
+      auto row_at = [&](int x) -> uint64_t {
         const int row = base + 32 * x + lane, i = S.row_of(row), g = row - i * S.group;
-        rows[x] = row < packed ? reinterpret_cast<uint64_t>(static_cast<const uint16_t *>(A.q) + (w.e.row0 + i) * A.q_row +
-                                                            (w.head * S.group + g) * A.q_head)
-                               : 0;
-      }
+        return row < packed ? reinterpret_cast<uint64_t>(static_cast<const uint16_t *>(A.q) + (w.e.row0 + i) * A.q_row +
+                                                         (w.head * S.group + g) * A.q_head)
+                            : 0;
+      };
       constexpr int kPer = D / 8, kRows = 32 / kPer;   // 16-byte parts of a row; rows a step
       const int c = lane % kPer, sub = lane / kPer;
       uint8_t *to = dst + (c >> 3) * 16384;
-      auto copy = [&](int x, int y, bool vec) {
+      auto copy = [&](uint64_t mine, int x, int y, bool vec) {
         const int rr = y * kRows + sub, r = 32 * x + rr;
-        const uint64_t from = __shfl_sync(0xffffffffu, rows[x], rr);
+        const uint64_t from = __shfl_sync(0xffffffffu, mine, rr);
         uint8_t *at = to + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         if (vec) {   // rows that are not there: no bytes read, zeros written
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(at)),
@@ -475,15 +462,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         }
       };
       if (A.q_vec) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll 8
-          for (int y = 0; y < kPer; ++y) copy(x, y, true);
-      } else {
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
 #pragma unroll 1
-          for (int y = 0; y < kPer; ++y) copy(x, y, false);
+        for (int x = 0; x < 4; ++x) {
+          const uint64_t mine = row_at(x);
+#pragma unroll 4
+          for (int y = 0; y < kPer; ++y) copy(mine, x, y, true);
+        }
+      } else {
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          const uint64_t mine = row_at(x);
+#pragma unroll 1
+          for (int y = 0; y < kPer; ++y) copy(mine, x, y, false);
+        }
       }
       cp_async_commit();
       const int first = w.first(), count = w.count(S);
