@@ -32,7 +32,7 @@ namespace paged {
 constexpr int kTilesTile = 256, kTilesHalf = 128, kTilesBlock = 128;
 constexpr int kTilesExtra = 1;   // a tile's start and end, in blocks
 constexpr int kTilesLeast = 3;   // units a piece has at least
-constexpr int kTurnAt = 5;   // of eight parts of its exponentials, those a half has added up when it passes its turn on
+constexpr int kTurnAt = 2;   // the quarter of its exponentials after which a half passes its turn on (1: 186 us, 2: 183, 3: 186)
 constexpr int kTilesThreads = 384;
 // Registers a thread after the split: 256 softmax threads x 216 + 128 others x
 // 72 = 384 x 168, what the block is launched with.
@@ -111,7 +111,23 @@ __device__ __forceinline__ void t_st32(uint32_t taddr, const uint32_t *u) {
         "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
       : "memory");
 }
-__device__ __forceinline__ void t_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void t_st16(uint32_t taddr, const uint32_t *u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]),
+        "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+      : "memory");
+}
+// This thread's TMEM loads are done; names 32 registers that they fill, so
+// that nothing reads those before.
+__device__ __forceinline__ void t_ld_wait(float *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+        "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+        "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+        "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+      ::"memory");
+}
 __device__ __forceinline__ void t_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Two FP32 operations an instruction.
@@ -554,7 +570,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         float s[128];
 #pragma unroll
         for (int x = 0; x < 4; ++x) t_ld32(t_s + x * 32, s + x * 32);
-        t_ld_wait();
+#pragma unroll
+        for (int x = 0; x < 4; ++x) t_ld_wait(s + x * 32);
         if constexpr (Z::kEarly) {
           t_before();
           __syncwarp();
@@ -595,7 +612,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
             for (int x = 0; x < D / 32; ++x) {
               float o[32];
               t_ld32(t_o + x * 32, o);
-              t_ld_wait();
+              t_ld_wait(o);
 #pragma unroll
               for (int y = 0; y < 32; ++y) o[y] *= a;
               t_st32(t_o + x * 32, reinterpret_cast<const uint32_t *>(o));
@@ -609,32 +626,22 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         // the same time, at half speed each, and then both wait at the same time.
         if (two && !wait(&bars.turn[h][warp & 3], turns - (h == 0 ? 1 : 0))) break;
         const float mc = m == -INFINITY ? 0.f : m * c;
-        // sixteen exponentials in flight while the sixteen before them are
-        // added up and packed
         const uint64_t c2 = f2(c, c), mc2 = f2(-mc, -mc);
         uint64_t sum[4] = {0, 0, 0, 0};
-        uint32_t p[32];
-        float e[2][16];
 #pragma unroll
-        for (int x = 0; x <= 8; ++x) {
-          if (x < 8) {
+        for (int x = 0; x < 4; ++x) {   // 32 at a time; the stores hold their order
+          uint32_t p[16];
 #pragma unroll
-            for (int y = 0; y < 8; ++y)
-              f2_split(f2_fma(f2(s[x * 16 + 2 * y], s[x * 16 + 2 * y + 1]), c2, mc2), s[x * 16 + 2 * y], s[x * 16 + 2 * y + 1]);
-#pragma unroll
-            for (int y = 0; y < 16; ++y) e[x & 1][y] = exp2_approx(s[x * 16 + y]);
+          for (int y = 0; y < 16; ++y) {
+            float a, b;
+            f2_split(f2_fma(f2(s[x * 32 + 2 * y], s[x * 32 + 2 * y + 1]), c2, mc2), a, b);
+            a = exp2_approx(a);
+            b = exp2_approx(b);
+            sum[y & 3] = f2_add(sum[y & 3], f2(a, b));
+            p[y] = E::pack(a, b);
           }
-          if (x > 0) {
-            const float *d = e[(x - 1) & 1];
-#pragma unroll
-            for (int y = 0; y < 8; ++y) {
-              sum[y & 3] = f2_add(sum[y & 3], f2(d[2 * y], d[2 * y + 1]));
-              p[((x - 1) & 3) * 8 + y] = E::pack(d[2 * y], d[2 * y + 1]);
-            }
-            if (x == 4) t_st32(t_p, p);
-            if (x == kTurnAt && two && lane == 0) mbar_arrive_count(&bars.turn[h ^ 1][warp & 3], 1);
-            if (x == 8) t_st32(t_p + 32, p);
-          }
+          t_st16(t_p + x * 16, p);
+          if (x == kTurnAt && two && lane == 0) mbar_arrive_count(&bars.turn[h ^ 1][warp & 3], 1);
         }
         turns += two ? 1 : 0;
         float l0, l1;
@@ -659,7 +666,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         for (int x = 0; x < D / 32; ++x) {
           float o[32];
           t_ld32(t_o + x * 32, o);
-          t_ld_wait();
+          t_ld_wait(o);
 #pragma unroll
           for (int y = 0; y < 8; ++y)
             __stcg(reinterpret_cast<float4 *>(part) + (x * 8 + y) * 128 + r,
@@ -703,7 +710,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         if (whole) {
           t_ld32(t_o + x * 64, o);
           t_ld32(t_o + x * 64 + 32, o + 32);
-          t_ld_wait();
+          t_ld_wait(o);
+          t_ld_wait(o + 32);
         } else if (write) {
           const float *p = A.parts + h * Z::kPartFloats;
 #pragma unroll
