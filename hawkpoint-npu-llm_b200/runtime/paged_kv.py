@@ -23,7 +23,7 @@ All index lists are int32 device tensors.  Pages are laid out
 ``rows`` gives a slot's K and V in plain order.
 
 Calls on one cache share its workspace: run them on one stream, or order the
-streams with events.
+streams with events, and make them from one thread at a time.
 """
 
 import ctypes
@@ -103,7 +103,7 @@ class PagedKVCache:
             lengths_dev=lengths.data_ptr())
         if n_pages == 1:
             p.page_stride = pool[0].numel() * 2
-        self._pool = ctypes.byref(p)
+        self._pool = ctypes.addressof(p)
         need = self._lib.hb_paged_workspace_bytes(self._pool)
         if need == 0:
             hb_lib.check(hb_lib.HB_ERR_INVALID_ARG)
@@ -113,10 +113,11 @@ class PagedKVCache:
         self._int32, self._float32 = torch.int32, torch.float32
         self._scale = self.head_dim ** -0.5
         self._empty = torch.empty_strided
-        self._current_device = torch.cuda.current_device
-        # torch's own accessor of the current stream's handle, without a Stream object where there is one
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        self._current_stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+        # the current device and the current stream's handle, by torch's own accessors where it has them
+        self._current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self._current_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                                       lambda index: torch.cuda.current_stream(index).cuda_stream)
+        self._attend, self._append = self._lib.hb_paged_attend, self._lib.hb_paged_append
         # what a call fills, and its addresses
         self._rows_buf, self._args_buf = bytearray(_ROWS.size), bytearray(max(_QUERY.size, _NEW.size))
         self._rows_at, self._args_at = (ctypes.addressof(ctypes.c_char.from_buffer(b)) for b in (self._rows_buf, self._args_buf))
@@ -138,12 +139,18 @@ class PagedKVCache:
             raise ValueError(f"{name} has {t.shape[0]} entries, not {n}")
         return t.data_ptr()
 
-    def _fill_rows(self, slots, row_start, rows, max_rows):
-        entries = slots.shape[0]
+    def _run(self, fn, layer, slots, row_start, rows, max_rows):
+        entries = len(slots)
         if max_rows < 0 or (entries == 0 and rows > 0):
             raise ValueError("max_rows must not be negative, and rows need an entry")
         _ROWS.pack_into(self._rows_buf, 0, self._list("slots", slots), self._list("row_start", row_start, entries + 1),
                         entries, rows, max_rows if max_rows < rows else rows, 0)
+        index = self._index
+        if self._current_device() != index:
+            return self._call(fn, layer, self._rows_at, self._args_at)
+        rc = fn(self._pool, layer, self._rows_at, self._args_at, self._current_stream(index))
+        if rc:
+            hb_lib.check(rc)
 
     def _heads(self, name, t, rows=None):
         """(shape, strides) of rows of heads."""
@@ -176,19 +183,18 @@ class PagedKVCache:
         if q_heads < 0:
             raise ValueError(f"qkv has fewer heads than the {2 * self.kv_heads} of k and v")
         table = cos.shape
-        for name, t in (("cos", cos), ("sin", sin)):
-            if t.dtype is not self._float32 or t.shape != table or len(table) != 2 or table[1] * 2 != d or (
-                    not t.is_contiguous() or t.device != self.device):
-                raise ValueError(f"{name} must be a contiguous float32 [positions, {d // 2}] on the cache's device, "
-                                 "cos and sin of one shape")
+        if len(table) != 2 or table[1] * 2 != d or sin.shape != table or (
+                cos.dtype is not self._float32 or sin.dtype is not self._float32 or cos.device != self.device
+                or sin.device != self.device or not (cos.is_contiguous() and sin.is_contiguous())):
+            raise ValueError(f"cos and sin must be contiguous float32 [positions, {d // 2}] on the cache's device, of one "
+                             "shape")
         if out is None:
             out, q_row, q_head = self._new_heads(rows, q_heads), q_heads * d, d
         else:
             _, (q_row, q_head, _) = self._heads("out", out, (rows, q_heads))
-        self._fill_rows(slots, row_start, rows, max_rows)
         _NEW.pack_into(self._args_buf, 0, qkv.data_ptr(), row_stride, out.data_ptr(), q_row, q_head, cos.data_ptr(),
                        sin.data_ptr(), table[0], q_heads)
-        self._call(self._lib.hb_paged_append, layer, self._rows_at, self._args_at)
+        self._run(self._append, layer, slots, row_start, rows, max_rows)
         return out
 
     def attend(self, layer, q, slots, row_start, max_rows, scale=None, window=0, out=None, lse=False):
@@ -203,10 +209,9 @@ class PagedKVCache:
         else:
             _, (o_row, o_head, _) = self._heads("out", out, (rows, heads))
         sums = self._empty((rows, heads), (heads, 1), dtype=self._float32, device=self.device) if lse else None
-        self._fill_rows(slots, row_start, rows, max_rows)
         _QUERY.pack_into(self._args_buf, 0, q.data_ptr(), q_row, q_head, out.data_ptr(), o_row, o_head,
                          sums.data_ptr() if lse else 0, heads, window, self._scale if scale is None else scale, 0)
-        self._call(self._lib.hb_paged_attend, layer, self._rows_at, self._args_at)
+        self._run(self._attend, layer, slots, row_start, rows, max_rows)
         return (out, sums) if lse else out
 
     # -- pages -----------------------------------------------------------------------
