@@ -1,6 +1,6 @@
 // hb_paged.cu -- the paged K/V cache operators of the C ABI: argument checks,
-// workspace and launches around hb_paged_rows.cuh (attention) and
-// hb_paged_ops.cuh (append and the page operators).
+// workspace and launches around hb_paged_rows.cuh and hb_paged_tiles.cuh
+// (attention) and hb_paged_ops.cuh (append and the page operators).
 #include <atomic>
 
 #include "hb_engine_impl.h"
@@ -13,6 +13,7 @@ namespace pg = hb::paged;
 namespace {
 
 constexpr int kMaxDevices = 64;
+constexpr int kMaxHeads = 1 << 16;   // q heads: products with them are 32-bit
 constexpr int kAppendMost = pg::kAppendRows;
 constexpr int kAppendBlocks = 8;
 
@@ -281,13 +282,15 @@ int hb_paged_attend(const hb_page_pool *pool, int layer, const hb_paged_rows *ro
   if (!q) return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_attend: query is NULL");
   if (q->q_heads < 1 || q->q_heads % pool->kv_heads)
     return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_attend: q_heads must be a positive multiple of kv_heads");
+  if (q->q_heads > kMaxHeads) return fail(nullptr, HB_ERR_UNSUPPORTED, "hb_paged_attend: at most %d q heads", kMaxHeads);
   if (!(q->scale > 0.f) || q->scale > 1e30f || q->window < 0)
     return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_attend: scale must be positive, window not negative");
   if (rows->rows == 0 || rows->entries == 0) return HB_OK;
   // the most units the call's line can have (16-row tiles), counted in 32 bits
   const double units = (static_cast<double>(rows->rows) * q->q_heads / pg::kRowsTile + pool->kv_heads * rows->entries) *
                        (pool->table_width + pg::kRowsExtra);
-  if (units >= 2e9) return fail(nullptr, HB_ERR_UNSUPPORTED, "hb_paged_attend: too many rows for the table's width in one call");
+  if (units >= 2e9 || static_cast<double>(rows->rows) * q->q_heads >= 2e9)   // nor more packed rows
+    return fail(nullptr, HB_ERR_UNSUPPORTED, "hb_paged_attend: too many rows for the table's width in one call");
   if (!q->q_dev || !q->out_dev) return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_attend: null pointer");
   if ((reinterpret_cast<uintptr_t>(q->q_dev) | reinterpret_cast<uintptr_t>(q->out_dev)) & 1)
     return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_attend: q and out must be element aligned");
@@ -339,6 +342,7 @@ int hb_paged_append(const hb_page_pool *pool, int layer, const hb_paged_rows *ro
   if (!n) return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_append: new rows are NULL");
   if (n->q_heads < 0 || n->rope_positions < 1)
     return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_append: q_heads must not be negative, rope_positions positive");
+  if (n->q_heads > kMaxHeads) return fail(nullptr, HB_ERR_UNSUPPORTED, "hb_paged_append: at most %d q heads", kMaxHeads);
   if (rows->rows == 0 || rows->entries == 0) return HB_OK;
   if (!n->qkv_dev || !n->cos_dev || !n->sin_dev || (n->q_heads > 0 && !n->q_dev))
     return fail(nullptr, HB_ERR_INVALID_ARG, "hb_paged_append: null pointer");

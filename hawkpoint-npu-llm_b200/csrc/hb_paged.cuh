@@ -28,7 +28,8 @@ struct Control {
   Ctrl ctrl;
   int status;    // HB_PAGED_* bits, cleared by hb_paged_status
   int copies;    // entries of the copy list
-  int pad[6];
+  int refused;   // a reserve or fork changed nothing since the status was read
+  int pad[5];
 };
 static_assert(sizeof(Control) == 64, "control block");
 

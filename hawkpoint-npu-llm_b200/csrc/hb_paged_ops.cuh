@@ -101,8 +101,8 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
         }
       }
       if (bad) atomicOr(&A.pool.control->status, bad);
-      // a reserve that ran out of pages left lengths and pages as they were: these are not this row's places
-      if (ld_volatile_int(&A.pool.control->status) & HB_PAGED_EXHAUSTED) pg = -1;
+      // a reserve or fork that was refused left lengths and pages as they were: these are not this row's places
+      if (ld_volatile_int(&A.pool.control->refused)) pg = -1;
       s_pos[i] = pos;
       s_page[i] = pg;
     }
@@ -285,7 +285,10 @@ __global__ void __launch_bounds__(kBookThreads) reserve_kernel(Pool P, Scratch X
     if (slots[b] >= 0 && slots[b] < P.n_slots) X.mark[slots[b]] = 0;
   __syncthreads();
   if (s_bad) {   // all or nothing
-    if (threadIdx.x == 0) atomicOr(&P.control->status, s_bad);
+    if (threadIdx.x == 0) {
+      atomicOr(&P.control->status, s_bad);
+      P.control->refused = 1;
+    }
     return;
   }
   for (int b = warp; b < n; b += 32) {
@@ -351,7 +354,10 @@ __global__ void __launch_bounds__(kBookThreads) fork_kernel(Pool P, Scratch X, c
   for (int b = threadIdx.x; b < n; b += kBookThreads)
     if (dst[b] >= 0 && dst[b] < P.n_slots) X.mark[dst[b]] = 0;
   if (s_bad || total > free) {   // all or nothing
-    if (threadIdx.x == 0) atomicOr(&P.control->status, s_bad ? s_bad : HB_PAGED_EXHAUSTED);
+    if (threadIdx.x == 0) {
+      atomicOr(&P.control->status, s_bad ? s_bad : HB_PAGED_EXHAUSTED);
+      P.control->refused = 1;
+    }
     return;
   }
   __syncthreads();

@@ -363,7 +363,9 @@ int hb_prefill_tc(hb_engine *engine, int slot, const int32_t *ids, int n, int st
  * workspace): one stream, or events between streams.  What only the device
  * can see -- an exhausted pool, an index out of range, a row without a page --
  * is not an error of the call: it does nothing there, sets a bit in the
- * workspace, and hb_paged_status reports it. */
+ * workspace, and hb_paged_status reports it.  After a reserve or fork that
+ * was refused appends write no K / V until the status has been read: the
+ * lengths they would go by were not updated. */
 enum { HB_ELEM_BF16 = 0, HB_ELEM_FP16 = 1 };
 enum {
   HB_PAGED_EXHAUSTED = 1,   /* reserve / fork found too few free pages and changed nothing */

@@ -652,6 +652,55 @@ def test_append_after_an_exhausted_reserve_writes_nothing():
 
 
 @gpu
+@pytest.mark.parametrize("refused", ["past the table", "slot twice", "fork past the source"])
+def test_append_after_a_refused_call_writes_nothing(refused):
+    """Lengths stayed as they were, so the rows' positions would be those of
+    rows that the slot holds already."""
+    torch = _torch()
+    from runtime.paged_kv import PagedKVCache
+
+    cache = PagedKVCache(1, 1, 64, 8, 2, 256)
+    cache.reserve(ints([0, 1]), ints([200, 20]))
+    cos, sin = tables(64, 256)
+    qkv = torch.ones((200, 3 * 64), dtype=torch.bfloat16, device="cuda")
+    cache.append(0, qkv, ints([0]), ints([0, 200]), 200, cos, sin)
+    before = cache.pool.clone()
+    if refused == "past the table":
+        cache.reserve(ints([0]), ints([60]))
+    elif refused == "slot twice":
+        cache.reserve(ints([0, 0]), ints([5, 5]))
+    else:
+        cache.fork(ints([1]), ints([0]), ints([21]))
+    cache.append(0, 2 * qkv[:60], ints([0]), ints([0, 60]), 60, cos, sin)
+    assert torch.equal(cache.pool, before)
+    with pytest.raises(hb_lib.HbError, match="out of range"):
+        cache.status()
+    cache.reserve(ints([0]), ints([5]))  # usable again once the status is read
+    cache.append(0, 2 * qkv[:5], ints([0]), ints([0, 5]), 5, cos, sin)
+    cache.status()
+    assert not torch.equal(cache.pool, before)
+
+
+def test_c_refusals_of_sizes_past_32_bits():
+    lib = hb_lib.load()
+    fake = 1 << 20
+    pool = ctypes.byref(hb_lib.HbPagePool(
+        pages_dev=fake, page_stride=16384, n_pages=4, layers=1, kv_heads=1, head_dim=64, element=0, n_slots=2,
+        table_width=1, table_dev=fake, refs_dev=fake, lengths_dev=fake, workspace_dev=fake, workspace_bytes=1 << 40))
+    attend = lambda heads, rows: lib.hb_paged_attend(  # noqa: E731
+        pool, 0, ctypes.byref(hb_lib.HbPagedRows(fake, fake, 1, rows, rows, 0)), ctypes.byref(hb_lib.HbPagedQuery(
+            q_dev=fake, q_row_stride=0, q_head_stride=0, out_dev=fake, out_row_stride=0, out_head_stride=0, q_heads=heads,
+            scale=1.0)), None)
+    assert attend((1 << 16) + 1, 1) == hb_lib.HB_ERR_UNSUPPORTED
+    assert attend(1 << 16, 1 << 15) == hb_lib.HB_ERR_UNSUPPORTED
+    assert attend(1, (1 << 31) - 1) == hb_lib.HB_ERR_UNSUPPORTED
+    assert lib.hb_paged_append(
+        pool, 0, ctypes.byref(hb_lib.HbPagedRows(fake, fake, 1, 1, 1, 0)), ctypes.byref(hb_lib.HbPagedNew(
+            qkv_dev=fake, qkv_row_stride=192, q_dev=fake, q_row_stride=64, q_head_stride=64, cos_dev=fake, sin_dev=fake,
+            rope_positions=8, q_heads=1 << 28)), None) == hb_lib.HB_ERR_UNSUPPORTED
+
+
+@gpu
 def test_copy_pages_within_and_between_pools():
     torch = _torch()
     from runtime.paged_kv import PagedKVCache
