@@ -183,19 +183,27 @@ int launch_copy(const hb_page_pool &p, void *to_pages, int to_n, const int *from
 
 // Which kernels an attention call launches: the rows kernel for entries of up
 // to 16 packed rows (its tile), the tiles kernel for the others, one of them
-// where the host's numbers say that it may have them all.  Where entries have
-// no more than a 16-row tile each on average and none is long, a second launch
-// costs more than the rows kernel loses on the few that have more (96 streams,
-// 12 of them with chunks of up to 32 x 3 packed rows: 37 us in one launch, 56
-// in two); all entries alike above 16 rows are the tiles kernel's.  A bound on
-// an entry's rows that is wrong costs time, not rows: a kernel launched alone
-// takes every entry.
+// where the host's numbers say that it may have them all.  The tiles kernel
+// costs a prologue and steps of 256 rows however few there are; the rows kernel
+// reads an entry's pages again for every 16 rows of it, which heads of 64 can
+// afford twice on average and heads of 128 hardly at all.  So the rows kernel
+// has the call alone if no entry has more than 8 of its tiles and the average
+// is at most 32 packed rows (heads of 64) or 8 (heads of 128).  Measured, rows
+// kernel alone / otherwise, us: heads of 64, 64 streams of 1024 with 21 rows
+// each 20.4 / 24.6, with 63 rows 30.6 / 24.9; 96 streams of 200 to 2000 of which
+// 12 have 126 rows (21.9 on average) 28.8 / 36.6.  Heads of 128: 64 streams with
+// 24 rows 104 / 75; 96 streams, 12 with 32 rows (7.5 on average) 102 / 105, 12
+// with 64 rows (11.5) 123 / 104.  All entries alike above that are the tiles
+// kernel's alone.  A bound on an entry's rows that is wrong costs time, not
+// rows: a kernel launched alone takes every entry.
 template <int D, class T>
 cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) {
   const pg::Batch &b = A.batch;
   const int64_t most = static_cast<int64_t>(max_rows) * A.shape.group;
-  const bool rows_only = most <= pg::kRowsTile ||
-                         (most <= 8 * pg::kRowsTile && static_cast<int64_t>(b.rows) * A.shape.group <= static_cast<int64_t>(b.entries) * pg::kRowsTile);
+  constexpr int kMean = D == 64 ? 2 * pg::kRowsTile : pg::kRowsTile / 2;
+  const bool rows_only =
+      most <= pg::kRowsTile || (most <= 8 * pg::kRowsTile &&
+                                static_cast<int64_t>(b.rows) * A.shape.group <= static_cast<int64_t>(b.entries) * kMean);
   const bool tiles_only = !rows_only && static_cast<int64_t>(b.entries) * max_rows == b.rows;
   const size_t line = pg::line_bytes(b.entries);
   A.few = rows_only ? INT32_MAX : tiles_only ? 0 : pg::kRowsTile;
