@@ -15,7 +15,7 @@ namespace {
 constexpr int kMaxDevices = 64;
 constexpr int kMaxHeads = 1 << 16;   // q heads: products with them are 32-bit
 constexpr int kAppendMost = pg::kAppendRows;
-constexpr int kAppendBlocks = 8;
+constexpr int kAppendBlocks = 8;   // blocks a multiprocessor, at most (4: 27.4 us for 24 prompts, 8: 27.5, 16: 29.7)
 
 // What a device's calls need to know, looked up on the first of them.
 struct DeviceInfo {

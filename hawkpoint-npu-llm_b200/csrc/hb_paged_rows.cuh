@@ -12,6 +12,12 @@
 // tcgen05 tile would be 128 rows for 16), with a running maximum and sum of
 // their own that are joined once a tile.  The weights are multiplied as a
 // high and a low half, so they lose nothing to the 16-bit V product.
+//
+// Measured: 48 streams of 4000 to 16,000 positions, 32 q heads on 8 of 128,
+// FP16: 290 us, 6.7 TB/s, a plain copy's rate.  128 streams of 200 to 4096,
+// 14 heads on 2 of 64, BF16: 33.5 us, 4.3 TB/s; about 8 us are launch, line,
+// the first pages and the last tiles' joins.  One such stream of 4032: 9.9 us,
+// all of it that latency.
 #pragma once
 
 #include "hb_paged.cuh"
@@ -20,8 +26,12 @@ namespace hb {
 namespace paged {
 
 constexpr int kRowsTile = 16;
-constexpr int kRowsExtra = 4;                       // a tile's start and end, in pages
-constexpr int kRowsLeast = 5;                       // units a piece has at least
+// A tile's start and end, in pages (2: 128 streams 36.2 us, a step that mixes
+// chunks and decoding 42; 4: 34.4, 37; 8: 34.4, 39).
+constexpr int kRowsExtra = 4;
+// Units a piece has at least: more and shorter pieces read a lone stream's pages
+// sooner and have more parts to join (3 and 5: 10.2 us, 8: 12.1).
+constexpr int kRowsLeast = 5;
 constexpr int kRowsWarps = 4;                       // consumer warps
 constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
 template <int D>
@@ -114,6 +124,8 @@ __device__ __forceinline__ bool store_row(const Attend &A, const Entry &e, int h
   return fine;
 }
 
+// Two blocks a multiprocessor with heads of 64 (three would have to keep parts
+// of O in memory), one with heads of 128, whose ring has the same bytes.
 template <int D, class T>
 __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kernel(const __grid_constant__ Attend A, int least) {
   using E = Elem<T>;

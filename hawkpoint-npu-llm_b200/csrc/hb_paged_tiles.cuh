@@ -13,15 +13,26 @@
 // What bounds it: with heads of 64 a step's 2 x 2.1 MFLOP take the tensor
 // pipe 512 cycles a half, its 16,384 exponentials the 16-a-cycle special
 // function units 1,024: the softmax is the bound, and the two halves take
-// turns so that one's MMAs run under the other's exponentials.  With heads of
-// 128 both take 1,024 cycles.  O is rescaled only when a row's maximum has
-// grown by more than 2^8 (the sum and O share the stale maximum, so the
-// result is the same), which after the first blocks is almost never.
+// turns so that one's MMAs run under the other's exponentials (193 us without
+// turns, 175 with).  With heads of 128 both take 1,024 cycles.  O is rescaled
+// only when a row's maximum has grown by more than 2^8 (the sum and O share
+// the stale maximum, so the result is the same), which after the first blocks
+// is almost never.
+//
+// Measured, BF16: four prompts of 3000 to 4096 positions, 14 q heads on 2 of
+// 64: 174.5 us, 547 TFLOP/s, 2.1 times the exponentials' 83 us; a step of both
+// halves takes 3,300 cycles, 2,050 of them the exponentials themselves, the
+// rest scores on their way from the MMA, their maximum, and the hand-over of
+// the turn.  Chunks of 200 to 512 rows of four prompts, 32 q heads on 8 of 128,
+// window 1024: 65 us, 405 TFLOP/s; some 11 blocks a multiprocessor there, so the
+// start (7 us to the first scores) and the joins weigh as much as the steps.
 //
 // Warps 0-3 and 4-7: the softmax of either half; warp 8: MMA issue; warp 9:
-// K and V; warps 10 and 11: the halves' q, a tile ahead.  One block a multiprocessor; the line of blocks is cut evenly
-// (hb_paged.cuh), a tile cut by a border is joined by the last of its pieces
-// to finish.
+// K and V; warps 10 and 11: the halves' q, a tile ahead.  One block a
+// multiprocessor; the line of blocks is cut evenly (hb_paged.cuh), a tile cut
+// by a border is joined by the last of its pieces to finish.  The weights are
+// rounded to 16 bits for the product with V, as the MMA wants them: their sum
+// is taken before, so a row's weights still add up to one within the rounding.
 #pragma once
 
 #include "hb_paged_rows.cuh"
@@ -30,9 +41,15 @@ namespace hb {
 namespace paged {
 
 constexpr int kTilesTile = 256, kTilesHalf = 128, kTilesBlock = 128;
-constexpr int kTilesExtra = 1;   // a tile's start and end, in blocks
-constexpr int kTilesLeast = 3;   // units a piece has at least
-constexpr int kTurnAt = 2;   // the quarter of its exponentials after which a half passes its turn on (1: 186 us, 2: 183, 3: 186)
+// A tile's start and end, in blocks (0: whole prompts 202 us; 1: 174.5; 2: the
+// same; 3: 177).
+constexpr int kTilesExtra = 1;
+// Units a piece has at least: fewer pieces for small calls, whose joins would
+// cost more than the blocks (2, 3 and 5 the same on calls that fill the GPU).
+constexpr int kTilesLeast = 3;
+// The quarter of its exponentials after which a half passes its turn on (when
+// first tried 1: 186 us, 2: 183, 3: 186).
+constexpr int kTurnAt = 2;
 constexpr int kTilesThreads = 384;
 // Registers a thread after the split: 256 softmax threads x 216 + 128 others x
 // 72 = 384 x 168, what the block is launched with.
@@ -287,247 +304,247 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == 9) {
-    // ---- loads: K(0), then K(j + 1), V(j), the order the MMAs use them in
-    int it = 0;
-    bool ok = true;
-    auto load = [&](bool is_v, int block, int pg0, int pg1) {
-      const int s = it % Z::kStages;
-      const uint32_t ph = static_cast<uint32_t>(it / Z::kStages) & 1u;
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[s], ph ^ 1u, ctrl, A.limit_ns, kWhereEmpty)) != 0;
-      if (!ok) return;
-      uint8_t *dst = ring + s * Z::kOperand;
-      int held[2];
-      uint32_t bytes = 0;
-      bool wrote = false;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        held[x] = (x ? pg1 : pg0) < 0 ? 0 : max(0, min(kPage, w.e.length - (2 * block + x) * kPage));
-        bytes += (D / 64) * held[x] * 128;
-        if (is_v && held[x] < kPage) {   // V where there is no position: zero, so that weight zero times it is zero
-          for (int h = 0; h < D / 64; ++h)
-            for (int y = held[x] * 128 + lane * 16; y < kBlockBytes; y += 512)
-              *reinterpret_cast<uint4 *>(dst + h * 16384 + x * kBlockBytes + y) = make_uint4(0, 0, 0, 0);
-          wrote = true;
-        }
-      }
-      if (wrote) {
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      if (lane == 0) {
-        if (bytes) mbar_arrive_expect_tx(&bars.full[s], bytes); else mbar_arrive_count(&bars.full[s], 1);
+    if (warp == 9) {
+      // ---- loads: K(0), then K(j + 1), V(j), the order the MMAs use them in
+      int it = 0;
+      bool ok = true;
+      auto load = [&](bool is_v, int block, int pg0, int pg1) {
+        const int s = it % Z::kStages;
+        const uint32_t ph = static_cast<uint32_t>(it / Z::kStages) & 1u;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[s], ph ^ 1u, ctrl, A.limit_ns, kWhereEmpty)) != 0;
+        if (!ok) return;
+        uint8_t *dst = ring + s * Z::kOperand;
+        int held[2];
+        uint32_t bytes = 0;
+        bool wrote = false;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          if (!held[x]) continue;
-          const uint8_t *src = kv_block(A, x ? pg1 : pg0, w.head) + (is_v ? D / 64 * kBlockBytes : 0);
-          for (int h = 0; h < D / 64; ++h)
-            bulk_g2s(dst + h * 16384 + x * kBlockBytes, src + h * kBlockBytes, held[x] * 128, &bars.full[s]);
+          held[x] = (x ? pg1 : pg0) < 0 ? 0 : max(0, min(kPage, w.e.length - (2 * block + x) * kPage));
+          bytes += (D / 64) * held[x] * 128;
+          if (is_v && held[x] < kPage) {   // V where there is no position: zero, so that weight zero times it is zero
+            for (int h = 0; h < D / 64; ++h)
+              for (int y = held[x] * 128 + lane * 16; y < kBlockBytes; y += 512)
+                *reinterpret_cast<uint4 *>(dst + h * 16384 + x * kBlockBytes + y) = make_uint4(0, 0, 0, 0);
+            wrote = true;
+          }
         }
-      }
-      __syncwarp();
-      ++it;
-    };
-    for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
-      const int first = w.first(), count = w.count(S);
-      int mine = -1, k0 = -1, k1 = -1, v0 = -1, v1 = -1;
-      // K(0), then K(j), V(j - 1) in turn, at last V(count - 1).  One place for
-      // all loads: the warps' loops share the instruction cache.
-#pragma unroll 1
-      for (int x = 0; x < 2 * count && ok; ++x) {
-        const bool last = x == 2 * count - 1, is_v = last || (x != 0 && (x & 1) == 0);
-        int block = last ? count - 1 : (x >> 1) - 1, p0 = last ? k0 : v0, p1 = last ? k1 : v1;
-        if (!is_v) {
-          block = (x + 1) >> 1;
-          if ((block & 15) == 0) mine = page_of(A.pool, w.e.slot, 2 * (first + block) + lane);
-          v0 = k0;
-          v1 = k1;
-          p0 = k0 = __shfl_sync(0xffffffffu, mine, 2 * (block & 15));
-          p1 = k1 = __shfl_sync(0xffffffffu, mine, 2 * (block & 15) + 1);
+        if (wrote) {
+          fence_proxy_async_smem();
+          __syncwarp();
         }
-        load(is_v, first + block, p0, p1);
-      }
-    }
-    for (int i = max(0, it - Z::kStages); i < it; ++i)   // nothing in flight when the block ends
-      mbar_wait_quiet(&bars.full[i % Z::kStages], static_cast<uint32_t>(i / Z::kStages) & 1u, A.limit_ns);
-  } else if (warp == 8) {
-    // ---- MMA issue
-    constexpr uint32_t kIdescS = tiles_idesc<T>(kTilesBlock, false), kIdescO = tiles_idesc<T>(D, true);
-    constexpr uint32_t kStep = Z::kOperand >> 4;
-    const uint32_t leader = t_leader();
-    const uint32_t q_lo = swizzled_lo(smem_u32(smem), 16), k_lo = swizzled_lo(smem_u32(ring), 16),
-                   v_lo = swizzled_lo(smem_u32(ring), 16384);
-    uint32_t it = 0;                // ring stages consumed
-    uint32_t n_q0 = 0, n_q1 = 0, n_s[2] = {0, 0};   // tiles and steps of either half so far
-    bool ok = true;
-    auto wait = [&](uint64_t *bar, uint32_t phase) {
-      ok = __all_sync(0xffffffffu, ok && t_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
-      return ok;
-    };
-    auto stage = [&](uint32_t i) { return i % Z::kStages; };
-    auto wait_ring = [&](uint32_t i) { return wait(&bars.full[stage(i)], i / Z::kStages); };
-    auto commit = [&](uint64_t *bar) { t_commit(smem_u32(bar), leader); };
-    // S of half h from its q buffer and the K in ring use i
-    auto mma_s = [&](int h, uint32_t buf, uint32_t i) {
-      t_after();
-      const uint32_t a = q_lo + (buf * 2 + h) * kStep, b = k_lo + stage(i) * kStep;
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-        t_mma_ss(Z::kS + h * 128, swizzled_desc(a + off), swizzled_desc(b + off), kIdescS, k != 0, leader);
-      }
-      commit(&bars.s_full[h]);
-    };
-    // O of half h from its P and the V in ring use i
-    auto mma_o = [&](int h, uint32_t i, uint32_t acc) {
-      t_after();
-      const uint32_t b = v_lo + stage(i) * kStep;
-#pragma unroll
-      for (int k = 0; k < kTilesBlock / 16; ++k)
-        t_mma_ts(Z::kO + h * D, Z::kP + h * Z::kPHalf + k * 8, swizzled_desc(b + k * (2048 >> 4)), kIdescO, k ? 1 : acc,
-                 leader);
-      commit(&bars.o_done[h]);
-    };
-    while (ok) {
-      const uint32_t buf0 = n_q0 % Z::kQ;
-      if (!wait(&bars.q_full[0][buf0], n_q0 / Z::kQ)) break;
-      const TileInfo &info = s_info[0][n_q0 % kInfoSlots];
-      // reductions over the warp, for results in uniform registers
-      const uint32_t count = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(info.count));
-      const bool two = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(info.two)) != 0;
-      if (count == 0) break;
-      // S is free: the last step's P of either half, which was waited for,
-      // was written after its S was read
-      ++n_q0;
-      const uint32_t buf1 = n_q1 % Z::kQ;
-      if (two) {
-        wait(&bars.q_full[1][buf1], n_q1 / Z::kQ);
-        ++n_q1;
-      }
-      // steps -1 (the first S alone), 0 .. count - 1: the next step's S, this
-      // one's O; one place for either, the warps' loops share the instruction cache
-#pragma unroll 1
-      for (int j = -1; ok && j < static_cast<int>(count); ++j) {
-        const bool next = j + 1 < static_cast<int>(count);
-        const uint32_t ik = it + (j < 0 ? 0 : 2 * j + 1), iv = next ? ik + 1 : ik;
-        if (!next) {   // every S of the tile is issued
-          commit(&bars.q_empty[0][buf0]);
-          if (two) commit(&bars.q_empty[1][buf1]);
-        }
-        if (next && !wait_ring(ik)) break;
-        if (Z::kEarly && next) {
-#pragma unroll 1
-          for (int h = 0; h < (two ? 2 : 1); ++h)
-            if (j < 0 || wait(&bars.s_read[h], n_s[h])) mma_s(h, h ? buf1 : buf0, ik);
-          commit(&bars.empty[stage(ik)]);
-        }
-        if (j >= 0 && !wait_ring(iv)) break;
-#pragma unroll 1
-        for (int h = 0; h < (two ? 2 : 1); ++h) {
-          if (j >= 0 && wait(&bars.p_full[h], n_s[h]++)) mma_o(h, iv, j != 0);
-          if (!Z::kEarly && next && ok) mma_s(h, h ? buf1 : buf0, ik);   // over the P just used: MMAs run in order
-        }
-        if (!Z::kEarly && next) commit(&bars.empty[stage(ik)]);
-        if (j >= 0) commit(&bars.empty[stage(iv)]);
-      }
-      it += 2 * count;
-    }
-    commit(&bars.done);   // after a give-up too: nothing in flight when TMEM is freed
-  } else {
-    // ---- warps 10, 11: the q rows of half h, a tile ahead of its softmax
-    const int h = warp - 10;
-    uint32_t n = 0;
-    bool ok = true;
-    while (ok) {
-      while (more && h >= halves()) more = w.next(A.pool, A.batch, S, line);
-      const int buf = n % Z::kQ;
-      ok = __all_sync(0xffffffffu, n < Z::kQ || mbar_wait(&bars.q_empty[h][buf], (n / Z::kQ - 1) & 1u, ctrl, A.limit_ns,
-                                                          kWhereEmpty)) != 0;
-      TileInfo &info = s_info[h][n % kInfoSlots];
-      if (!more || !ok) {
         if (lane == 0) {
-          info.count = 0;
+          if (bytes) mbar_arrive_expect_tx(&bars.full[s], bytes); else mbar_arrive_count(&bars.full[s], 1);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!held[x]) continue;
+            const uint8_t *src = kv_block(A, x ? pg1 : pg0, w.head) + (is_v ? D / 64 * kBlockBytes : 0);
+            for (int h = 0; h < D / 64; ++h)
+              bulk_g2s(dst + h * 16384 + x * kBlockBytes, src + h * kBlockBytes, held[x] * 128, &bars.full[s]);
+          }
+        }
+        __syncwarp();
+        ++it;
+      };
+      for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
+        const int first = w.first(), count = w.count(S);
+        int mine = -1, k0 = -1, k1 = -1, v0 = -1, v1 = -1;
+        // K(0), then K(j), V(j - 1) in turn, at last V(count - 1).  One place for
+        // all loads: the warps' loops share the instruction cache.
+#pragma unroll 1
+        for (int x = 0; x < 2 * count && ok; ++x) {
+          const bool last = x == 2 * count - 1, is_v = last || (x != 0 && (x & 1) == 0);
+          int block = last ? count - 1 : (x >> 1) - 1, p0 = last ? k0 : v0, p1 = last ? k1 : v1;
+          if (!is_v) {
+            block = (x + 1) >> 1;
+            if ((block & 15) == 0) mine = page_of(A.pool, w.e.slot, 2 * (first + block) + lane);
+            v0 = k0;
+            v1 = k1;
+            p0 = k0 = __shfl_sync(0xffffffffu, mine, 2 * (block & 15));
+            p1 = k1 = __shfl_sync(0xffffffffu, mine, 2 * (block & 15) + 1);
+          }
+          load(is_v, first + block, p0, p1);
+        }
+      }
+      for (int i = max(0, it - Z::kStages); i < it; ++i)   // nothing in flight when the block ends
+        mbar_wait_quiet(&bars.full[i % Z::kStages], static_cast<uint32_t>(i / Z::kStages) & 1u, A.limit_ns);
+    } else if (warp == 8) {
+      // ---- MMA issue
+      constexpr uint32_t kIdescS = tiles_idesc<T>(kTilesBlock, false), kIdescO = tiles_idesc<T>(D, true);
+      constexpr uint32_t kStep = Z::kOperand >> 4;
+      const uint32_t leader = t_leader();
+      const uint32_t q_lo = swizzled_lo(smem_u32(smem), 16), k_lo = swizzled_lo(smem_u32(ring), 16),
+                     v_lo = swizzled_lo(smem_u32(ring), 16384);
+      uint32_t it = 0;                // ring stages consumed
+      uint32_t n_q0 = 0, n_q1 = 0, n_s[2] = {0, 0};   // tiles and steps of either half so far
+      bool ok = true;
+      auto wait = [&](uint64_t *bar, uint32_t phase) {
+        ok = __all_sync(0xffffffffu, ok && t_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
+        return ok;
+      };
+      auto stage = [&](uint32_t i) { return i % Z::kStages; };
+      auto wait_ring = [&](uint32_t i) { return wait(&bars.full[stage(i)], i / Z::kStages); };
+      auto commit = [&](uint64_t *bar) { t_commit(smem_u32(bar), leader); };
+      // S of half h from its q buffer and the K in ring use i
+      auto mma_s = [&](int h, uint32_t buf, uint32_t i) {
+        t_after();
+        const uint32_t a = q_lo + (buf * 2 + h) * kStep, b = k_lo + stage(i) * kStep;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+          t_mma_ss(Z::kS + h * 128, swizzled_desc(a + off), swizzled_desc(b + off), kIdescS, k != 0, leader);
+        }
+        commit(&bars.s_full[h]);
+      };
+      // O of half h from its P and the V in ring use i
+      auto mma_o = [&](int h, uint32_t i, uint32_t acc) {
+        t_after();
+        const uint32_t b = v_lo + stage(i) * kStep;
+#pragma unroll
+        for (int k = 0; k < kTilesBlock / 16; ++k)
+          t_mma_ts(Z::kO + h * D, Z::kP + h * Z::kPHalf + k * 8, swizzled_desc(b + k * (2048 >> 4)), kIdescO, k ? 1 : acc,
+                   leader);
+        commit(&bars.o_done[h]);
+      };
+      while (ok) {
+        const uint32_t buf0 = n_q0 % Z::kQ;
+        if (!wait(&bars.q_full[0][buf0], n_q0 / Z::kQ)) break;
+        const TileInfo &info = s_info[0][n_q0 % kInfoSlots];
+        // reductions over the warp, for results in uniform registers
+        const uint32_t count = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(info.count));
+        const bool two = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(info.two)) != 0;
+        if (count == 0) break;
+        // S is free: the last step's P of either half, which was waited for,
+        // was written after its S was read
+        ++n_q0;
+        const uint32_t buf1 = n_q1 % Z::kQ;
+        if (two) {
+          wait(&bars.q_full[1][buf1], n_q1 / Z::kQ);
+          ++n_q1;
+        }
+        // steps -1 (the first S alone), 0 .. count - 1: the next step's S, this
+        // one's O; one place for either, the warps' loops share the instruction cache
+#pragma unroll 1
+        for (int j = -1; ok && j < static_cast<int>(count); ++j) {
+          const bool next = j + 1 < static_cast<int>(count);
+          const uint32_t ik = it + (j < 0 ? 0 : 2 * j + 1), iv = next ? ik + 1 : ik;
+          if (!next) {   // every S of the tile is issued
+            commit(&bars.q_empty[0][buf0]);
+            if (two) commit(&bars.q_empty[1][buf1]);
+          }
+          if (next && !wait_ring(ik)) break;
+          if (Z::kEarly && next) {
+#pragma unroll 1
+            for (int h = 0; h < (two ? 2 : 1); ++h)
+              if (j < 0 || wait(&bars.s_read[h], n_s[h])) mma_s(h, h ? buf1 : buf0, ik);
+            commit(&bars.empty[stage(ik)]);
+          }
+          if (j >= 0 && !wait_ring(iv)) break;
+#pragma unroll 1
+          for (int h = 0; h < (two ? 2 : 1); ++h) {
+            if (j >= 0 && wait(&bars.p_full[h], n_s[h]++)) mma_o(h, iv, j != 0);
+            if (!Z::kEarly && next && ok) mma_s(h, h ? buf1 : buf0, ik);   // over the P just used: MMAs run in order
+          }
+          if (!Z::kEarly && next) commit(&bars.empty[stage(ik)]);
+          if (j >= 0) commit(&bars.empty[stage(iv)]);
+        }
+        it += 2 * count;
+      }
+      commit(&bars.done);   // after a give-up too: nothing in flight when TMEM is freed
+    } else {
+      // ---- warps 10, 11: the q rows of half h, a tile ahead of its softmax
+      const int h = warp - 10;
+      uint32_t n = 0;
+      bool ok = true;
+      while (ok) {
+        while (more && h >= halves()) more = w.next(A.pool, A.batch, S, line);
+        const int buf = n % Z::kQ;
+        ok = __all_sync(0xffffffffu, n < Z::kQ || mbar_wait(&bars.q_empty[h][buf], (n / Z::kQ - 1) & 1u, ctrl, A.limit_ns,
+                                                            kWhereEmpty)) != 0;
+        TileInfo &info = s_info[h][n % kInfoSlots];
+        if (!more || !ok) {
+          if (lane == 0) {
+            info.count = 0;
+            mbar_arrive_count(&bars.q_full[h][buf], 1);
+            mbar_arrive_count(&bars.i_full[h][n % kInfoSlots], 1);
+          }
+          break;
+        }
+        const int packed = w.e.n * S.group, base = w.t * kTilesTile + h * kTilesHalf;
+        uint8_t *dst = smem + (buf * 2 + h) * Z::kOperand;
+        // a lane 16 bytes, D / 8 lanes a row; each lane finds one of 32 rows
+        auto row_at = [&](int x) -> uint64_t {
+          const int row = base + 32 * x + lane, i = S.row_of(row), g = row - i * S.group;
+          return row < packed ? reinterpret_cast<uint64_t>(static_cast<const uint16_t *>(A.q) + (w.e.row0 + i) * A.q_row +
+                                                           (w.head * S.group + g) * A.q_head)
+                              : 0;
+        };
+        constexpr int kPer = D / 8, kRows = 32 / kPer;   // 16-byte parts of a row; rows a step
+        const int c = lane % kPer, sub = lane / kPer;
+        uint8_t *to = dst + (c >> 3) * 16384;
+        auto copy = [&](uint64_t mine, int x, int y, bool vec) {
+          const int rr = y * kRows + sub, r = 32 * x + rr;
+          const uint64_t from = __shfl_sync(0xffffffffu, mine, rr);
+          uint8_t *at = to + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+          if (vec) {   // rows that are not there: no bytes read, zeros written
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(at)),
+                         "l"(from != 0 ? from + c * 16 : reinterpret_cast<uint64_t>(A.q)), "r"(from != 0 ? 16 : 0)
+                         : "memory");
+          } else {
+            *reinterpret_cast<uint4 *>(at) =
+                from != 0 ? load8<false>(reinterpret_cast<const uint16_t *>(from) + c * 8) : make_uint4(0, 0, 0, 0);
+          }
+        };
+        if (A.q_vec) {
+#pragma unroll 1
+          for (int x = 0; x < 4; ++x) {
+            const uint64_t mine = row_at(x);
+#pragma unroll 4
+            for (int y = 0; y < kPer; ++y) copy(mine, x, y, true);
+          }
+        } else {
+#pragma unroll 1
+          for (int x = 0; x < 4; ++x) {
+            const uint64_t mine = row_at(x);
+#pragma unroll 1
+            for (int y = 0; y < kPer; ++y) copy(mine, x, y, false);
+          }
+        }
+        cp_async_commit();
+        const int first = w.first(), count = w.count(S);
+        bool hole = false;   // whether a page of the piece's blocks is missing
+        for (int p = 2 * first + lane; p < 2 * (first + count); p += 32)
+          hole |= p * kPage < w.e.length && page_of(A.pool, w.e.slot, p) < 0;
+        hole = __any_sync(0xffffffffu, hole) != 0;
+        if (lane == 0) {
+          info.count = count;
+          info.first = first;
+          info.base = base;
+          info.packed = packed;
+          info.row0 = w.e.row0;
+          info.n = w.e.n;
+          info.length = w.e.length;
+          info.slot = w.e.slot;
+          info.head = w.head;
+          info.two = halves() == 2;
+          info.whole = w.whole();
+          info.opens = w.opens();
+          info.hole = hole;
+          if (!w.whole()) {
+            info.c0 = cut.of(w.tile_u + S.extra);
+            info.c1 = cut.of(w.tile_u + w.units - 1);
+          }
+        }
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
           mbar_arrive_count(&bars.q_full[h][buf], 1);
           mbar_arrive_count(&bars.i_full[h][n % kInfoSlots], 1);
         }
-        break;
+        ++n;
+        more = w.next(A.pool, A.batch, S, line);
       }
-      const int packed = w.e.n * S.group, base = w.t * kTilesTile + h * kTilesHalf;
-      uint8_t *dst = smem + (buf * 2 + h) * Z::kOperand;
-      // a lane 16 bytes, D / 8 lanes a row; each lane finds one of 32 rows
-      auto row_at = [&](int x) -> uint64_t {
-        const int row = base + 32 * x + lane, i = S.row_of(row), g = row - i * S.group;
-        return row < packed ? reinterpret_cast<uint64_t>(static_cast<const uint16_t *>(A.q) + (w.e.row0 + i) * A.q_row +
-                                                         (w.head * S.group + g) * A.q_head)
-                            : 0;
-      };
-      constexpr int kPer = D / 8, kRows = 32 / kPer;   // 16-byte parts of a row; rows a step
-      const int c = lane % kPer, sub = lane / kPer;
-      uint8_t *to = dst + (c >> 3) * 16384;
-      auto copy = [&](uint64_t mine, int x, int y, bool vec) {
-        const int rr = y * kRows + sub, r = 32 * x + rr;
-        const uint64_t from = __shfl_sync(0xffffffffu, mine, rr);
-        uint8_t *at = to + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        if (vec) {   // rows that are not there: no bytes read, zeros written
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(at)),
-                       "l"(from != 0 ? from + c * 16 : reinterpret_cast<uint64_t>(A.q)), "r"(from != 0 ? 16 : 0)
-                       : "memory");
-        } else {
-          *reinterpret_cast<uint4 *>(at) =
-              from != 0 ? load8<false>(reinterpret_cast<const uint16_t *>(from) + c * 8) : make_uint4(0, 0, 0, 0);
-        }
-      };
-      if (A.q_vec) {
-#pragma unroll 1
-        for (int x = 0; x < 4; ++x) {
-          const uint64_t mine = row_at(x);
-#pragma unroll 4
-          for (int y = 0; y < kPer; ++y) copy(mine, x, y, true);
-        }
-      } else {
-#pragma unroll 1
-        for (int x = 0; x < 4; ++x) {
-          const uint64_t mine = row_at(x);
-#pragma unroll 1
-          for (int y = 0; y < kPer; ++y) copy(mine, x, y, false);
-        }
-      }
-      cp_async_commit();
-      const int first = w.first(), count = w.count(S);
-      bool hole = false;   // whether a page of the piece's blocks is missing
-      for (int p = 2 * first + lane; p < 2 * (first + count); p += 32)
-        hole |= p * kPage < w.e.length && page_of(A.pool, w.e.slot, p) < 0;
-      hole = __any_sync(0xffffffffu, hole) != 0;
-      if (lane == 0) {
-        info.count = count;
-        info.first = first;
-        info.base = base;
-        info.packed = packed;
-        info.row0 = w.e.row0;
-        info.n = w.e.n;
-        info.length = w.e.length;
-        info.slot = w.e.slot;
-        info.head = w.head;
-        info.two = halves() == 2;
-        info.whole = w.whole();
-        info.opens = w.opens();
-        info.hole = hole;
-        if (!w.whole()) {
-          info.c0 = cut.of(w.tile_u + S.extra);
-          info.c1 = cut.of(w.tile_u + w.units - 1);
-        }
-      }
-      cp_async_wait_all();
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive_count(&bars.q_full[h][buf], 1);
-        mbar_arrive_count(&bars.i_full[h][n % kInfoSlots], 1);
-      }
-      ++n;
-      more = w.next(A.pool, A.batch, S, line);
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTilesRegs));
     // ---- softmax of half h, a thread a row

@@ -133,14 +133,14 @@ class PagedKVCache:
             hb_lib.check(rc)
 
     def _list(self, name, t, n=None):
-        if t.dtype is not self._int32 or t.dim() != 1 or not t.is_contiguous() or t.device != self.device:
+        if t.dtype is not self._int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != self._index:
             raise ValueError(f"{name} must be a contiguous one-dimensional int32 tensor on the cache's device")
-        if n is not None and t.shape[0] != n:
-            raise ValueError(f"{name} has {t.shape[0]} entries, not {n}")
+        if n is not None and t.numel() != n:
+            raise ValueError(f"{name} has {t.numel()} entries, not {n}")
         return t.data_ptr()
 
     def _run(self, fn, layer, slots, row_start, rows, max_rows):
-        entries = len(slots)
+        entries = slots.numel()
         if max_rows < 0 or (entries == 0 and rows > 0):
             raise ValueError("max_rows must not be negative, and rows need an entry")
         _ROWS.pack_into(self._rows_buf, 0, self._list("slots", slots), self._list("row_start", row_start, entries + 1),
@@ -154,7 +154,7 @@ class PagedKVCache:
 
     def _heads(self, name, t, rows=None):
         """(shape, strides) of rows of heads."""
-        if t.dtype is not self.dtype or t.dim() != 3 or t.device != self.device:
+        if t.dtype is not self.dtype or t.dim() != 3 or t.get_device() != self._index:
             raise ValueError(f"{name} must be [rows, heads, {self.head_dim}] of {self.dtype} on the cache's device")
         shape, stride = t.shape, t.stride()
         if shape[2] != self.head_dim or stride[2] != 1:
@@ -174,7 +174,7 @@ class PagedKVCache:
         heads + 2 kv heads) * head_dim]; ``cos`` / ``sin`` float32 [positions,
         head_dim / 2].  Returns the rotated q [rows, q heads, head_dim]."""
         d = self.head_dim
-        if qkv.dtype is not self.dtype or qkv.dim() != 2 or qkv.device != self.device:
+        if qkv.dtype is not self.dtype or qkv.dim() != 2 or qkv.get_device() != self._index:
             raise ValueError(f"qkv must be [rows, heads * {d}] of {self.dtype} on the cache's device")
         (rows, cols), (row_stride, col_stride) = qkv.shape, qkv.stride()
         if cols % d or col_stride != 1:
@@ -184,8 +184,8 @@ class PagedKVCache:
             raise ValueError(f"qkv has fewer heads than the {2 * self.kv_heads} of k and v")
         table = cos.shape
         if len(table) != 2 or table[1] * 2 != d or sin.shape != table or (
-                cos.dtype is not self._float32 or sin.dtype is not self._float32 or cos.device != self.device
-                or sin.device != self.device or not (cos.is_contiguous() and sin.is_contiguous())):
+                cos.dtype is not self._float32 or sin.dtype is not self._float32 or cos.get_device() != self._index
+                or sin.get_device() != self._index or not (cos.is_contiguous() and sin.is_contiguous())):
             raise ValueError(f"cos and sin must be contiguous float32 [positions, {d // 2}] on the cache's device, of one "
                              "shape")
         if out is None:

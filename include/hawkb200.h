@@ -391,7 +391,8 @@ typedef struct hb_page_pool {
 /* The rows of a call: entry b is slot slots_dev[b] with rows row_start_dev[b]
  * .. row_start_dev[b + 1] (ascending from 0; entries + 1 values); row i of its n stands at
  * position lengths[slot] - n + i.  At most 1024 entries.  max_rows: the most
- * rows of an entry (an upper bound; it chooses kernels, never results). */
+ * rows of an entry (it chooses kernels and so the rounding of weights; every
+ * row is done whatever it says). */
 typedef struct hb_paged_rows {
   const int32_t *slots_dev, *row_start_dev;
   int32_t entries, rows, max_rows, reserved0;
@@ -428,10 +429,11 @@ int hb_paged_status(const hb_page_pool *pool, int32_t *status, void *stream);
 /* out = softmax(scale q.K + mask) V over one layer's pages: a row sees the
  * mapped positions up to its own, with a window the last `window` of them.  A
  * row that sees none gives zeros and an lse of -infinity.  Positions that a row does
- * not see never reach it, whatever they hold.  Scores, sums and the running
- * maximum are FP32; the weights are rounded to the element type for the
- * product with V where an entry has more than 16 rows of one kv head, else
- * kept to twice its bits; out is rounded once. */
+ * not see never reach it, whatever they hold (a row that meets infinities or
+ * NaN is done once more, slowly).  Scores, sums and the running maximum are
+ * FP32; for the product with V the weights are rounded to the element type in
+ * calls with long chunks, else kept to twice its bits; out is rounded once.
+ * out must not overlap q. */
 int hb_paged_attend(const hb_page_pool *pool, int layer, const hb_paged_rows *rows, const hb_paged_query *query,
                     void *stream);
 /* Rotates the rows' q and k (rotate-half RoPE with each row's position, the
