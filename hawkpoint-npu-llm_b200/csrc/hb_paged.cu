@@ -163,21 +163,28 @@ bool vec_ok(const void *base, int64_t a, int64_t b, unsigned bytes = 16) {
   return ((reinterpret_cast<uintptr_t>(base) | static_cast<uintptr_t>(a * 2) | static_cast<uintptr_t>(b * 2)) & (bytes - 1)) == 0;
 }
 
-// The copy kernel after a books kernel, launched early.
-int launch_copy(const hb_page_pool &p, void *to_pages, int to_n, const int *from, const int *to, const int *held,
-                const int *copies, int n, const int *map, int grid, cudaStream_t st) {
+// A launch that may begin while the kernel before it on the stream ends (every
+// kernel here waits for that one first).
+template <class... P, class... X>
+cudaError_t launch(void (*kernel)(P...), int grid, int block, size_t smem, cudaStream_t st, const X &...args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+int launch_copy(const hb_page_pool &p, void *to_pages, int to_n, const int *from, const int *to, const int *held,
+                const int *copies, int n, const int *map, int grid, cudaStream_t st) {
   const int blocks = static_cast<int>(layer_bytes(p) * p.layers / pg::kBlockBytes);
-  HB_CUDA(nullptr, cudaLaunchKernelEx(&cfg, pg::copy_kernel, pool_view(p), static_cast<uint8_t *>(to_pages), to_n, from, to,
-                                      held, copies, n, blocks, map));
+  HB_CUDA(nullptr, launch(pg::copy_kernel, grid, 256, 0, st, pool_view(p), static_cast<uint8_t *>(to_pages), to_n, from, to, held,
+                          copies, n, blocks, map));
   return HB_OK;
 }
 
@@ -211,28 +218,17 @@ cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) 
     A.shape.tile = pg::kRowsTile;
     A.shape.block = pg::kPage;
     A.shape.extra = pg::kRowsExtra;
-    pg::paged_rows_kernel<D, T><<<rows_pieces(D, sms), pg::kRowsThreads, pg::RowsSize<D>::kSmem + line, st>>>(A, pg::kRowsLeast);
+    const cudaError_t err = launch(pg::paged_rows_kernel<D, T>, rows_pieces(D, sms), pg::kRowsThreads,
+                                   pg::RowsSize<D>::kSmem + line, st, A, pg::kRowsLeast);
+    if (err != cudaSuccess || rows_only) return err;
   }
-  if (!rows_only) {
-    A.shape.tile = pg::kTilesTile;
-    A.shape.block = pg::kTilesBlock;
-    A.shape.extra = pg::kTilesExtra;
-    A.arrived = A.arrived2;
-    A.parts = A.parts2;
-    // beside the rows kernel, whose blocks leave first (it reads nothing of it)
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(sms);
-    cfg.blockDim = dim3(pg::kTilesThreads);
-    cfg.dynamicSmemBytes = pg::TilesSize<D>::kSmem + line;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = tiles_only ? 0 : 1;
-    return cudaLaunchKernelEx(&cfg, pg::paged_tiles_kernel<D, T>, A, pg::kTilesLeast);
-  }
-  return cudaGetLastError();
+  A.shape.tile = pg::kTilesTile;
+  A.shape.block = pg::kTilesBlock;
+  A.shape.extra = pg::kTilesExtra;
+  A.arrived = A.arrived2;
+  A.parts = A.parts2;
+  A.beside = !tiles_only;   // the rows kernel's blocks leave first; it reads nothing of that one's
+  return launch(pg::paged_tiles_kernel<D, T>, sms, pg::kTilesThreads, pg::TilesSize<D>::kSmem + line, st, A, pg::kTilesLeast);
 }
 
 template <int D, class T>
@@ -241,11 +237,8 @@ cudaError_t launch_append(const pg::Append &A, bool vec, int grid, cudaStream_t 
   const int parts = (A.q_heads + 2 * A.pool.kv_heads) * (D / 16);
   const int threads = parts >= pg::kAppendThreads ? pg::kAppendThreads
                                                   : (pg::kAppendThreads / parts * parts + 31) / 32 * 32;
-  if (vec)
-    pg::paged_append_kernel<D, T, true><<<grid, threads, 0, st>>>(A);
-  else
-    pg::paged_append_kernel<D, T, false><<<grid, threads, 0, st>>>(A);
-  return cudaGetLastError();
+  return vec ? launch(pg::paged_append_kernel<D, T, true>, grid, threads, 0, st, A)
+             : launch(pg::paged_append_kernel<D, T, false>, grid, threads, 0, st, A);
 }
 
 }  // namespace
@@ -400,8 +393,7 @@ int hb_pages_reserve(const hb_page_pool *pool, int n, const int32_t *slots_dev, 
   const Regions r = regions(*pool);
   const pg::Scratch x = scratch_view(*pool, r);
   const pg::Pool v = pool_view(*pool);
-  pg::reserve_kernel<<<1, pg::kBookThreads, 0, st>>>(v, x, slots_dev, counts_dev, n);
-  HB_CUDA(nullptr, cudaGetLastError());
+  HB_CUDA(nullptr, launch(pg::reserve_kernel, 1, pg::kBookThreads, 0, st, v, x, slots_dev, counts_dev, n));
   return launch_copy(*pool, pool->pages_dev, pool->n_pages, x.from, x.to, x.held, &v.control->copies, 0, nullptr, sms, st);
 }
 
@@ -418,8 +410,7 @@ int hb_pages_fork(const hb_page_pool *pool, int n, const int32_t *src_dev, const
   const Regions r = regions(*pool);
   const pg::Scratch x = scratch_view(*pool, r);
   const pg::Pool v = pool_view(*pool);
-  pg::fork_kernel<<<1, pg::kBookThreads, 0, st>>>(v, x, src_dev, dst_dev, counts_dev, n);
-  HB_CUDA(nullptr, cudaGetLastError());
+  HB_CUDA(nullptr, launch(pg::fork_kernel, 1, pg::kBookThreads, 0, st, v, x, src_dev, dst_dev, counts_dev, n));
   // a warp an 8 KB block to copy, as far as the GPU holds them at once
   const int64_t most = (static_cast<int64_t>(n) * (layer_bytes(*pool) * pool->layers / pg::kBlockBytes) + 7) / 8;
   return launch_copy(*pool, pool->pages_dev, pool->n_pages, x.from, x.to, x.held, &v.control->copies, 0, nullptr,
@@ -434,8 +425,7 @@ int hb_pages_free(const hb_page_pool *pool, int n, const int32_t *slots_dev, voi
   if (!slots_dev) return fail(nullptr, HB_ERR_INVALID_ARG, "hb_pages_free: null pointer");
   int sms = 0;
   if ((rc = device_info("hb_pages_free", &sms))) return rc;
-  pg::free_kernel<<<(n + 3) / 4, 128, 0, static_cast<cudaStream_t>(stream)>>>(pool_view(*pool), slots_dev, n);
-  HB_CUDA(nullptr, cudaGetLastError());
+  HB_CUDA(nullptr, launch(pg::free_kernel, (n + 3) / 4, 128, 0, static_cast<cudaStream_t>(stream), pool_view(*pool), slots_dev, n));
   return HB_OK;
 }
 
@@ -449,8 +439,7 @@ int hb_pages_compact(const hb_page_pool *pool, int32_t *map_dev, void *stream) {
   const Regions r = regions(*pool);
   const pg::Scratch x = scratch_view(*pool, r);
   const pg::Pool v = pool_view(*pool);
-  pg::compact_kernel<<<1, pg::kBookThreads, 0, st>>>(v, x, map_dev);
-  HB_CUDA(nullptr, cudaGetLastError());
+  HB_CUDA(nullptr, launch(pg::compact_kernel, 1, pg::kBookThreads, 0, st, v, x, map_dev));
   return launch_copy(*pool, pool->pages_dev, pool->n_pages, x.from, x.to, x.held, &v.control->copies, 0, map_dev, 8 * sms, st);
 }
 

@@ -64,6 +64,15 @@ __device__ __forceinline__ Entry entry_of(const Pool &P, const Batch &B, int b) 
   return e;
 }
 
+// Every kernel here is launched early (programmatic launch): its blocks take
+// their places while the kernel before it ends, wait for it and what it wrote,
+// and let the next one do the same.  Waiting comes first, so that at most two
+// kernels of a stream are under way.
+__device__ __forceinline__ void grid_begin() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ---- division of an attention call --------------------------------------------
 // The rows of an entry and the q heads of a kv head's group are packed into
 // tiles of `tile` rows: packed row r is row r / group, head r % group.  A
@@ -313,7 +322,7 @@ struct Elem<__half> {
 template <bool VEC>
 __device__ __forceinline__ uint4 load8(const uint16_t *p) {
   if constexpr (VEC) {
-    return __ldg(reinterpret_cast<const uint4 *>(p));
+    return *reinterpret_cast<const uint4 *>(p);   // not as read-only data: nothing goes ahead of grid_begin
   } else {
     uint32_t w[4];
 #pragma unroll
@@ -356,6 +365,7 @@ struct Attend {
   float scale, scale_log2;         // of the scores; times log2(e)
   int q_vec, o_vec;                // q rows / out rows are 16-byte aligned
   int o_wide;                      // 32-byte aligned
+  int beside;                      // the tiles kernel runs beside the rows kernel of the same call
   int few;                         // entries of up to this many packed rows are the rows kernel's, others the tiles'
   float *parts;                    // joined tiles: per piece two parts
   int *arrived;                    // per piece, zero between launches

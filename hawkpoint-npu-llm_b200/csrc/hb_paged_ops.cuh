@@ -67,6 +67,7 @@ __device__ __forceinline__ void rope8(const uint4 &x0, const uint4 &x1, const fl
 template <int D, class T, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ Append A) {
   __shared__ int s_pos[kAppendRows], s_page[kAppendRows];
+  grid_begin();
   const int row0 = blockIdx.x * A.block_rows, rows = min(A.block_rows, A.batch.rows - row0);
   // a thread keeps its part of a head (8 dims of either half) and takes every
   // `step`-th row, the next one's reads ahead
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
     int first = 0, n = A.batch.entries;
     while (n > 1) {
       const int stride = (n + 31) / 32, i = first + lane * stride;
-      const bool in = lane * stride < n && __ldg(A.batch.row_start + i) <= row0;
+      const bool in = lane * stride < n && A.batch.row_start[i] <= row0;
       const int k = max(0, 31 - __clz(__ballot_sync(0xffffffffu, in)));   // the last that starts at or before the row
       first += k * stride;
       n = min(stride, n - k * stride);
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
     for (int i = lane; i < rows; i += 32) {
       const int row = row0 + i;
       int b = first;
-      while (b + 1 < A.batch.entries && __ldg(A.batch.row_start + b + 1) <= row) ++b;
+      while (b + 1 < A.batch.entries && A.batch.row_start[b + 1] <= row) ++b;
       const Entry e = entry_of(A.pool, A.batch, b);
       int pos = e.length - e.n + row - e.row0, pg = -1, bad = 0;
       if (row < e.row0 || row >= e.row0 + e.n || e.slot < 0 || pos < 0) {
@@ -249,7 +250,7 @@ constexpr int kKeep = -2;   // stage: the page stays
 // entry order; the written part of a shared page is copied first.
 __global__ void __launch_bounds__(kBookThreads) reserve_kernel(Pool P, Scratch X, const int *slots, const int *counts,
                                                                int n) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the copy kernel's blocks may take their places
+  grid_begin();
   __shared__ int s_sums[32], s_bad;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
@@ -336,7 +337,7 @@ constexpr int kStageInts = 8192;
 // last page go to the lowest pages that were free before the call.
 __global__ void __launch_bounds__(kBookThreads) fork_kernel(Pool P, Scratch X, const int *src, const int *dst,
                                                             const int *counts, int n) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the copy kernel's blocks may take their places
+  grid_begin();
   __shared__ int s_sums[32], s_bad, s_stage[kStageInts];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
@@ -398,6 +399,7 @@ __global__ void __launch_bounds__(kBookThreads) fork_kernel(Pool P, Scratch X, c
 
 // hb_pages_free: a warp a slot.  A slot named twice is freed once.
 __global__ void __launch_bounds__(128) free_kernel(Pool P, const int *slots, int n) {
+  grid_begin();
   const int b = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (b >= n) return;
   const int slot = slots[b];
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(128) free_kernel(Pool P, const int *slots, int
 // hb_pages_compact: of L live pages the k-th with an index of L or more goes
 // to the k-th free index below L.  map[page] = its new index, -1 for a free one.
 __global__ void __launch_bounds__(kBookThreads) compact_kernel(Pool P, Scratch X, int *map) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the copy kernel's blocks may take their places
+  grid_begin();
   __shared__ int s_sums[32];
   int live = 0;
   for (int base = 0; base < P.n_pages; base += 4 * kBookThreads) {
@@ -473,7 +475,7 @@ __global__ void __launch_bounds__(kBookThreads) compact_kernel(Pool P, Scratch X
 __global__ void __launch_bounds__(256) copy_kernel(Pool P, uint8_t *to_pages, int to_n, const int *from, const int *to,
                                                    const int *held, const int *copies, int n, int blocks,
                                                    const int *map) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");   // the copy list is complete
+  grid_begin();   // the copy list is complete
   if (map != nullptr) {
     const int64_t entries = static_cast<int64_t>(P.n_slots) * P.width;
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < entries; i += gridDim.x * 256ll) {

@@ -135,7 +135,6 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
   __shared__ int s_valid[Z::kStages];
   __shared__ float s_m[kRowsWarps][kRowsTile], s_l[kRowsWarps][kRowsTile];
   __shared__ int s_bad[kRowsTile], s_last;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the tiles kernel of the same call may start
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Shape S = A.shape;
   const Line line = line_at(smem + Z::kSmem, A.batch.entries);
@@ -149,6 +148,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
     fence_mbar_init();
   }
   if (threadIdx.x < kRowsTile) s_bad[threadIdx.x] = 0;
+  grid_begin();
   fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group <= A.few; });
   const Cut cut(line.prefix[A.batch.entries], gridDim.x, least);
   if (static_cast<int>(blockIdx.x) >= cut.pieces) return;

@@ -284,6 +284,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     mbar_init(&bars.done, 1);
     fence_mbar_init();
   }
+  // beside the rows kernel, which began when what was before it had ended
+  if (!A.beside) grid_begin();
   fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group > A.few; });
   const Cut cut(line.prefix[A.batch.entries], gridDim.x, least);
   if (static_cast<int>(blockIdx.x) >= cut.pieces) {
