@@ -57,7 +57,7 @@ int device_info(const char *who, int *sms) {
 }
 
 // The pieces an attention call is cut into at most: resident blocks.
-constexpr int kMaxSms = 160;
+constexpr int kMaxSms = pg::kTilesPieces;
 int rows_pieces(int head_dim, int sms) { return head_dim == 64 ? 2 * sms : sms; }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -78,7 +78,7 @@ Regions regions(const hb_page_pool &p) {
   };
   r.mark = take(slots * 4);
   r.arrived = take(2 * kMaxSms * 4);
-  r.arrived2 = take(2 * kMaxSms * 4);
+  r.arrived2 = take(2 * 2 * pg::kTilesPieces * 4);
   r.need = take(slots * 4);
   r.off = take(slots * 4);
   r.fresh = take(pages * 4);

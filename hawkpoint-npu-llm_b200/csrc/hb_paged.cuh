@@ -80,7 +80,8 @@ __device__ __forceinline__ void grid_begin() {
 // (one at least, so that a tile without any is still written), and `extra`
 // units for its start and end.  The units of all tiles, entry by entry, head
 // by head, are one line that the thread blocks cut into equal pieces, so ragged
-// lengths leave none idle; a tile cut by a border is joined from its parts.
+// lengths leave none idle; a tile cut by a border is joined from its parts, in
+// the pieces' order, so that results do not depend on who joins.
 struct Shape {
   int group, width, window, tile, block, extra;
   uint32_t group_inv;   // 2^32 / group, rounded down (at most 2^32 - 1)
@@ -287,6 +288,13 @@ struct Cut {
 __device__ __forceinline__ int arrive_acq_rel(int *p) {
   int v;
   asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
+// Another thread's count, ordered before what is read after it.
+__device__ __forceinline__ int load_acquire(const int *p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
 

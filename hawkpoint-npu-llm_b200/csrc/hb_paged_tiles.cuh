@@ -30,7 +30,9 @@
 // Warps 0-3 and 4-7: the softmax of either half; warp 8: MMA issue; warp 9:
 // K and V; warps 10 and 11: the halves' q, a tile ahead.  One block a
 // multiprocessor; the line of blocks is cut evenly (hb_paged.cuh), a tile cut
-// by a border is joined by the last of its pieces to finish.  The weights are
+// by a border is joined by the last of its pieces to get to its end, which
+// keeps its own part in TMEM (all parts through memory: chunks 65 us instead
+// of 58, prompts 172 instead of 165).  The weights are
 // rounded to 16 bits for the product with V, as the MMA wants them: their sum
 // is taken before, so a row's weights still add up to one within the rounding.
 #pragma once
@@ -51,6 +53,8 @@ constexpr int kTilesLeast = 3;
 // first tried 1: 186 us, 2: 183, 3: 186).
 constexpr int kTurnAt = 2;
 constexpr int kTilesThreads = 384;
+constexpr int kTilesPieces = 160;   // blocks of a launch at most
+
 // Registers a thread after the split: 256 softmax threads x 216 + 128 others x
 // 72 = 384 x 168, what the block is launched with.
 constexpr int kTilesRegs = 216, kOtherRegs = 72;
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   __shared__ TilesBars bars;
   __shared__ uint32_t s_tmem;
   __shared__ TileInfo s_info[2][kInfoSlots];
-  __shared__ int s_last[2];
+  __shared__ int s_last[2], s_seen[2];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *ring = smem + 2 * Z::kQ * Z::kOperand;   // behind the q of either half, kQ tiles
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -598,20 +602,24 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         }
         const int j0 = (first + j) * kTilesBlock;
         if (hole || j0 + kTilesBlock - 1 > all_hi || j0 < all_lo) {
-          int hi = pos - j0;   // sees x <= hi
-          if (hole || S.window > 0) {
-            int lo = S.window > 0 ? hi - S.window : -1;   // and x > lo
-            if (hole) {
-              if (page_of(A.pool, info.slot, 2 * (first + j)) < 0) lo = max(lo, 63);
-              if (page_of(A.pool, info.slot, 2 * (first + j) + 1) < 0) hi = min(hi, 63);
-            }
-#pragma unroll
-            for (int x = 0; x < 128; ++x)
-              if (x <= lo) s[x] = -INFINITY;
+          // sees lo < x <= hi: a bit a position, which predicates are made from
+          // eight at a time (comparisons took twice the instructions)
+          const int hi = pos - j0, lo = S.window > 0 ? hi - S.window : -1;
+          bool gone[2] = {false, false};
+          if (hole) {
+            gone[0] = page_of(A.pool, info.slot, 2 * (first + j)) < 0;
+            gone[1] = page_of(A.pool, info.slot, 2 * (first + j) + 1) < 0;
           }
 #pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (x > hi) s[x] = -INFINITY;
+          for (int x = 0; x < 4; ++x) {
+            const int top = hi - 32 * x, under = lo - 32 * x;
+            uint32_t sees = top >= 31 ? ~0u : top < 0 ? 0u : (2u << top) - 1u;
+            if (under >= 0) sees &= under >= 31 ? 0u : ~1u << under;
+            if (gone[x >> 1]) sees = 0;
+#pragma unroll
+            for (int y = 0; y < 32; ++y)
+              if (!(sees >> y & 1u)) s[32 * x + y] = -INFINITY;
+          }
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -675,50 +683,74 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       t_after();
       const bool whole = info.whole != 0;
       constexpr int64_t kTwo = 2 * Z::kPartFloats;   // a part has two halves
-      bool write = in;
-      int c0 = 0, c1 = -1;
+      int c0 = 0, c1 = -1, own = 0;
+      float own_m = 0.f;   // before the parts are joined
       if (!whole) {
-        // a tile that other pieces share: leave this part, and the last of
-        // them to arrive joins all parts in order; [D / 4][128] of 4 floats
-        float *part = A.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (info.opens ? 1 : 0)) * kTwo + h * Z::kPartFloats;
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-          float o[32];
-          t_ld32(t_o + x * 32, o);
-          t_ld_wait(o);
-#pragma unroll
-          for (int y = 0; y < 8; ++y)
-            __stcg(reinterpret_cast<float4 *>(part) + (x * 8 + y) * 128 + r,
-                   make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]));
-        }
-        __stcg(part + 128 * D + r, m);
-        __stcg(part + 128 * (D + 1) + r, l);
-        if (!half_sync()) break;   // the half's part is written
+        // A tile that other pieces share.  All but the last of them to get here
+        // leave their parts ([D / 4][128] of 4 floats) and say so; that one
+        // waits for the parts and joins them with its own, which stays in TMEM,
+        // in the pieces' order.
         c0 = info.c0;
         c1 = info.c1;
-        if (r == 0) {
-          s_last[h] = arrive_acq_rel(&A.arrived[2 * c0 + h]) == c1 - c0;
-          if (s_last[h]) A.arrived[2 * c0 + h] = 0;
-        }
+        own = blockIdx.x;
+        int *arrived = A.arrived + 2 * c0 + h, *left = arrived + 2 * kTilesPieces;
+        if (r == 0) s_last[h] = atomicAdd(arrived, 1) == c1 - c0;
         if (!half_sync()) break;
-        write = write && s_last[h] != 0;
-        if (!half_sync()) break;   // s_last is read
-        if (write) {
-          const float *p = A.parts + h * Z::kPartFloats + 128 * D + r;
-          m = -INFINITY;
-          l = 0.f;
-#pragma unroll 4
-          for (int k = c0; k <= c1; ++k) {
-            const float *pk = p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo;
-            const float pm = __ldcg(pk), pl = __ldcg(pk + 128), nm = fmaxf(m, pm), use = nm == -INFINITY ? 0.f : nm;
-            l = l * exp2_approx((m - use) * c) + pl * exp2_approx((pm - use) * c);
-            m = nm;
+        if (s_last[h] == 0) {
+          float *part = A.parts + (static_cast<int64_t>(own) * 2 + (info.opens ? 1 : 0)) * kTwo + h * Z::kPartFloats;
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            float o[32];
+            t_ld32(t_o + x * 32, o);
+            t_ld_wait(o);
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+              __stcg(reinterpret_cast<float4 *>(part) + (x * 8 + y) * 128 + r,
+                     make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]));
           }
+          __stcg(part + 128 * D + r, m);
+          __stcg(part + 128 * (D + 1) + r, l);
+          if (!half_sync()) break;   // the half's part is written
+          if (r == 0) arrive_acq_rel(left);
+          t_before();   // as below
+          continue;
         }
+        if (r == 0) {
+          const uint64_t start = globaltimer_ns();
+          bool seen = true;
+          while (seen && load_acquire(left) < c1 - c0) {   // they are being written
+            if (ld_volatile_int(&ctrl->abort)) {
+              seen = false;
+            } else if (globaltimer_ns() - start > A.limit_ns) {
+              if (atomicCAS(&ctrl->err, 0, kErrTimeout) == 0) atomicExch(&ctrl->err_where, kWhereFull);
+              atomicExch(&ctrl->abort, 1);
+              seen = false;
+            }
+          }
+          if (seen) {
+            *arrived = 0;
+            *left = 0;
+          }
+          s_seen[h] = seen;
+        }
+        if (!half_sync() || s_seen[h] == 0) break;
+        const float *p = A.parts + h * Z::kPartFloats + 128 * D + r;
+        const float om = m, ol = l;
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll 4
+        for (int k = c0; k <= c1; ++k) {
+          const float *pk = p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo;
+          const float pm = k == own ? om : __ldcg(pk), pl = k == own ? ol : __ldcg(pk + 128);
+          const float nm = fmaxf(m, pm), use = nm == -INFINITY ? 0.f : nm;
+          l = l * exp2_approx((m - use) * c) + pl * exp2_approx((pm - use) * c);
+          m = nm;
+        }
+        own_m = om;
       }
       const int g = row - i * S.group, qh = info.head * S.group + g;
       const int64_t orow = info.row0 + i;
-      if (write && A.lse != nullptr)
+      if (in && A.lse != nullptr)
         A.lse[orow * A.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, A.scale, log2_approx(l) * 0.6931471805599453f);
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T *out = static_cast<T *>(A.out) + orow * A.o_row + qh * A.o_head;
@@ -731,27 +763,43 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
           t_ld32(t_o + x * 64 + 32, o + 32);
           t_ld_wait(o);
           t_ld_wait(o + 32);
-        } else if (write) {
+        } else {
           const float *p = A.parts + h * Z::kPartFloats;
+          const float use = m == -INFINITY ? 0.f : m;
 #pragma unroll
           for (int y = 0; y < 64; ++y) o[y] = 0.f;
+          // parts [c0, own), this one, the others
+#pragma unroll 1
+          for (int side = 0; side < 2; ++side) {
+            if (side == 1) {
+              const float f = exp2_approx((own_m - use) * c);
+#pragma unroll
+              for (int z = 0; z < 64; z += 32) {
+                float v[32];
+                t_ld32(t_o + x * 64 + z, v);
+                t_ld_wait(v);
+#pragma unroll
+                for (int y = 0; y < 32; ++y) o[z + y] = fmaf(v[y], f, o[z + y]);
+              }
+            }
 #pragma unroll 2
-          for (int k = c0; k <= c1; ++k) {
-            const float *pk = p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo;
-            const float f = exp2_approx((__ldcg(pk + 128 * D + r) - (m == -INFINITY ? 0.f : m)) * c);
-            float4 v[16];
+            for (int k = side ? own + 1 : c0; k < (side ? c1 + 1 : own); ++k) {
+              const float *pk = p + (k * 2 + (k == c0 ? 1 : 0)) * kTwo;
+              const float f = exp2_approx((__ldcg(pk + 128 * D + r) - use) * c);
+              float4 v[16];
 #pragma unroll
-            for (int y = 0; y < 16; ++y) v[y] = __ldcg(reinterpret_cast<const float4 *>(pk) + (x * 16 + y) * 128 + r);
+              for (int y = 0; y < 16; ++y) v[y] = __ldcg(reinterpret_cast<const float4 *>(pk) + (x * 16 + y) * 128 + r);
 #pragma unroll
-            for (int y = 0; y < 16; ++y) {
-              o[4 * y] = fmaf(v[y].x, f, o[4 * y]);
-              o[4 * y + 1] = fmaf(v[y].y, f, o[4 * y + 1]);
-              o[4 * y + 2] = fmaf(v[y].z, f, o[4 * y + 2]);
-              o[4 * y + 3] = fmaf(v[y].w, f, o[4 * y + 3]);
+              for (int y = 0; y < 16; ++y) {
+                o[4 * y] = fmaf(v[y].x, f, o[4 * y]);
+                o[4 * y + 1] = fmaf(v[y].y, f, o[4 * y + 1]);
+                o[4 * y + 2] = fmaf(v[y].z, f, o[4 * y + 2]);
+                o[4 * y + 3] = fmaf(v[y].w, f, o[4 * y + 3]);
+              }
             }
           }
         }
-        if (write) {
+        if (in) {
           uint32_t u[32];
 #pragma unroll
           for (int y = 0; y < 32; ++y) {
