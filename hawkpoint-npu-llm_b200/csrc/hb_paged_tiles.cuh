@@ -477,42 +477,31 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         }
         const int packed = w.e.n * S.group, base = w.t * kTilesTile + h * kTilesHalf;
         uint8_t *dst = smem + (buf * 2 + h) * Z::kOperand;
-        // a lane 16 bytes, D / 8 lanes a row; each lane finds one of 32 rows
-        auto row_at = [&](int x) -> uint64_t {
-          const int row = base + 32 * x + lane, i = S.row_of(row), g = row - i * S.group;
-          return row < packed ? reinterpret_cast<uint64_t>(static_cast<const uint16_t *>(A.q) + (w.e.row0 + i) * A.q_row +
-                                                           (w.head * S.group + g) * A.q_head)
-                              : 0;
-        };
-        constexpr int kPer = D / 8, kRows = 32 / kPer;   // 16-byte parts of a row; rows a step
-        const int c = lane % kPer, sub = lane / kPer;
-        uint8_t *to = dst + (c >> 3) * 16384;
-        auto copy = [&](uint64_t mine, int x, int y, bool vec) {
-          const int rr = y * kRows + sub, r = 32 * x + rr;
-          const uint64_t from = __shfl_sync(0xffffffffu, mine, rr);
-          uint8_t *at = to + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-          if (vec) {   // rows that are not there: no bytes read, zeros written
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(at)),
-                         "l"(from != 0 ? from + c * 16 : reinterpret_cast<uint64_t>(A.q)), "r"(from != 0 ? 16 : 0)
-                         : "memory");
+        // two lanes a row, 16 bytes of it each a step: a warp alone pays for every
+        // instruction, and a row is found once (a lane a row reads half sectors:
+        // prompts 169 us; four lanes a row 167; two 165)
+        constexpr int kLanes = 2, kRows = 32 / kLanes;
+        const int part = lane % kLanes;
+#pragma unroll 1
+        for (int x = 0; x < kTilesHalf; x += kRows) {
+          const int r = x + lane / kLanes, row = base + r, i = S.row_of(row), g = row - i * S.group;
+          const bool there = row < packed;   // else no bytes are read and zeros written
+          const uint16_t *from = static_cast<const uint16_t *>(A.q) + part * 8 +
+                                 (there ? (w.e.row0 + i) * A.q_row + (w.head * S.group + g) * A.q_head : 0);
+          uint8_t *to = dst + r * 128;
+          const int at = (part ^ (r & 7)) << 4;
+          if (A.q_vec) {
+#pragma unroll
+            for (int c = 0; c < D / 8; c += kLanes)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                               smem_u32(to) + ((c >> 3) * 16384 + (at ^ (c & 7) << 4))),
+                           "l"(from + c * 8), "r"(there ? 16 : 0)
+                           : "memory");
           } else {
-            *reinterpret_cast<uint4 *>(at) =
-                from != 0 ? load8<false>(reinterpret_cast<const uint16_t *>(from) + c * 8) : make_uint4(0, 0, 0, 0);
-          }
-        };
-        if (A.q_vec) {
 #pragma unroll 1
-          for (int x = 0; x < 4; ++x) {
-            const uint64_t mine = row_at(x);
-#pragma unroll 4
-            for (int y = 0; y < kPer; ++y) copy(mine, x, y, true);
-          }
-        } else {
-#pragma unroll 1
-          for (int x = 0; x < 4; ++x) {
-            const uint64_t mine = row_at(x);
-#pragma unroll 1
-            for (int y = 0; y < kPer; ++y) copy(mine, x, y, false);
+            for (int c = 0; c < D / 8; c += kLanes)
+              *reinterpret_cast<uint4 *>(to + (c >> 3) * 16384 + (at ^ (c & 7) << 4)) =
+                  there ? load8<false>(from + c * 8) : make_uint4(0, 0, 0, 0);
           }
         }
         cp_async_commit();
