@@ -7,10 +7,10 @@
 // of the low and the high half of a head each, so that the rotation's two
 // results are two 16-byte stores into the page's blocks; the next row's reads
 // are in flight under them.  RoPE is FP32 with unfused products, rounded once.
-// Measured, 14 q heads on 2 of 64, BF16: 24 prompts, 29,000 rows, 27.5 us,
+// Measured, 14 q heads on 2 of 64, BF16: 24 prompts, 29,000 rows, 27 us,
 // 4.9 TB/s, three quarters of a plain copy's rate: four rows in flight a
 // thread instead of two need registers that halve the threads (52 us and
-// more).  One row 2.9 us on the device, a launch.
+// more).  One row 2.4 us on the device, a launch.
 //
 // The page operators keep the pool's books on the device, so that a serving
 // loop neither waits for them nor uploads tables, and can be captured: one
@@ -18,10 +18,10 @@
 // latency, a handful of block scans, is the cost) and leaves a copy list that
 // a second kernel, launched early, works off with the whole GPU at HBM rate.
 // A new page is always the lowest free one, so results do not depend on the
-// order threads run in.  Measured: a fork of one stream 7.9 us (two launches
+// order threads run in.  Measured: a fork of one stream 7.4 us (two launches
 // and the books' four phases); of 64, 49 MB of partial pages copied, 18 us;
 // compaction of 1.1 GB 189 us, 5.9 TB/s of 6.5; free and reserve for 32
-// slots 9.6 us.  Books and copies as one launch, the blocks waiting for a
+// slots 8.4 us.  Books and copies as one launch, the blocks waiting for a
 // flag, cost 1.3 us less of the host and 3.1 us more on the device.
 #pragma once
 

@@ -13,28 +13,29 @@
 // What bounds it: with heads of 64 a step's 2 x 2.1 MFLOP take the tensor
 // pipe 512 cycles a half, its 16,384 exponentials the 16-a-cycle special
 // function units 1,024: the softmax is the bound, and the two halves take
-// turns so that one's MMAs run under the other's exponentials (193 us without
-// turns, 175 with).  With heads of 128 both take 1,024 cycles.  O is rescaled
+// turns so that one's MMAs run under the other's exponentials (when first
+// tried, 193 us without turns, 175 with).  With heads of 128 both take 1,024 cycles.  O is rescaled
 // only when a row's maximum has grown by more than 2^8 (the sum and O share
 // the stale maximum, so the result is the same), which after the first blocks
 // is almost never.
 //
 // Measured, BF16: four prompts of 3000 to 4096 positions, 14 q heads on 2 of
-// 64: 174.5 us, 547 TFLOP/s, 2.1 times the exponentials' 83 us; a step of both
+// 64: 162 us, 588 TFLOP/s, 2.0 times the exponentials' 83 us; a step of both
 // halves takes 3,300 cycles, 2,050 of them the exponentials themselves, the
 // rest scores on their way from the MMA, their maximum, and the hand-over of
 // the turn.  Chunks of 200 to 512 rows of four prompts, 32 q heads on 8 of 128,
-// window 1024: 65 us, 405 TFLOP/s; some 11 blocks a multiprocessor there, so the
-// start (7 us to the first scores) and the joins weigh as much as the steps.
+// window 1024: 54 us, 485 TFLOP/s; a multiprocessor has some 12 steps of 3,900
+// cycles there (P lies over S, so a half's next S waits for its P V), and the
+// start (7 us to the first scores) and the joins weigh as much as they do.
 //
 // Warps 0-3 and 4-7: the softmax of either half; warp 8: MMA issue; warp 9:
 // K and V; warps 10 and 11: the halves' q, a tile ahead.  One block a
 // multiprocessor; the line of blocks is cut evenly (hb_paged.cuh), a tile cut
 // by a border is joined by the last of its pieces to get to its end, which
 // keeps its own part in TMEM (all parts through memory: chunks 65 us instead
-// of 58, prompts 172 instead of 165).  The weights are
-// rounded to 16 bits for the product with V, as the MMA wants them: their sum
-// is taken before, so a row's weights still add up to one within the rounding.
+// of 58, prompts 172 instead of 165).  The weights are rounded to 16 bits for
+// the product with V, as the MMA wants them; their sum is of what they were
+// before, in FP32.
 #pragma once
 
 #include "hb_paged_rows.cuh"
@@ -43,14 +44,14 @@ namespace hb {
 namespace paged {
 
 constexpr int kTilesTile = 256, kTilesHalf = 128, kTilesBlock = 128;
-// A tile's start and end, in blocks (0: whole prompts 202 us; 1: 174.5; 2: the
-// same; 3: 177).
-constexpr int kTilesExtra = 1;
+// A tile's start and end, in blocks (0: whole prompts 190 us, chunks 58; 1:
+// 164.7, 55; 2: 162, 54; 3: 166, 54).
+constexpr int kTilesExtra = 2;
 // Units a piece has at least: fewer pieces for small calls, whose joins would
 // cost more than the blocks (2, 3 and 5 the same on calls that fill the GPU).
 constexpr int kTilesLeast = 3;
-// The quarter of its exponentials after which a half passes its turn on (when
-// first tried 1: 186 us, 2: 183, 3: 186).
+// The quarter of its exponentials after which a half passes its turn on (1:
+// 166.5 us, 2: 164.7, 3: 167.8).
 constexpr int kTurnAt = 2;
 constexpr int kTilesThreads = 384;
 constexpr int kTilesPieces = 160;   // blocks of a launch at most
