@@ -53,14 +53,22 @@ struct Entry {
   int row0, n, length, slot;   // slot -1: none (its rows see nothing)
 };
 
+// What an earlier kernel may have written.  The attention kernels read it past
+// L1 (PAST): the tiles kernel beside a rows kernel begins without a wait of its own.
+template <bool PAST, class T>
+__device__ __forceinline__ T read(const T *p) {
+  return PAST ? __ldcg(p) : *p;
+}
+
 // Entry b with every index held inside its array.
+template <bool PAST = false>
 __device__ __forceinline__ Entry entry_of(const Pool &P, const Batch &B, int b) {
   Entry e;
-  e.row0 = min(max(B.row_start[b], 0), B.rows);
-  e.n = min(max(B.row_start[b + 1], e.row0), B.rows) - e.row0;
-  e.slot = B.slots[b];
+  e.row0 = min(max(read<PAST>(B.row_start + b), 0), B.rows);
+  e.n = min(max(read<PAST>(B.row_start + b + 1), e.row0), B.rows) - e.row0;
+  e.slot = read<PAST>(B.slots + b);
   if (e.slot < 0 || e.slot >= P.n_slots) e.slot = -1;
-  e.length = e.slot < 0 ? 0 : max(P.lengths[e.slot], 0);
+  e.length = e.slot < 0 ? 0 : max(read<PAST>(P.lengths + e.slot), 0);
   return e;
 }
 
@@ -137,7 +145,7 @@ __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const S
   for (int b0 = warp * 32; b0 < B.entries; b0 += blockDim.x) {
     const int b = b0 + lane;
     Entry e{0, 0, 0, -1};
-    if (b < B.entries) line.entry[b] = e = entry_of(P, B, b);
+    if (b < B.entries) line.entry[b] = e = entry_of<true>(P, B, b);
     const int tiles = b < B.entries && take(e) ? tiles_of(S, e) : 0;
     int u = 0;
     if (tiles <= 4)
@@ -334,7 +342,8 @@ __device__ __forceinline__ uint4 load8(const uint16_t *p) {
   } else {
     uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = static_cast<uint32_t>(p[2 * k]) | static_cast<uint32_t>(p[2 * k + 1]) << 16;
+    for (int k = 0; k < 4; ++k)
+      w[k] = static_cast<uint32_t>(__ldcg(p + 2 * k)) | static_cast<uint32_t>(__ldcg(p + 2 * k + 1)) << 16;
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
@@ -387,9 +396,10 @@ __device__ __forceinline__ const uint8_t *kv_block(const Attend &A, int page, in
 }
 
 // Page `j` of a slot, -1 where none is mapped.
+template <bool PAST = false>
 __device__ __forceinline__ int page_of(const Pool &P, int slot, int j) {
   if (slot < 0 || j < 0 || j >= P.width) return -1;
-  const int pg = P.table[static_cast<int64_t>(slot) * P.width + j];
+  const int pg = read<PAST>(P.table + static_cast<int64_t>(slot) * P.width + j);
   return pg >= 0 && pg < P.n_pages ? pg : -1;
 }
 
@@ -407,14 +417,14 @@ __device__ __noinline__ void row_alone(const Attend &A, const Entry &e, int head
   float qf[kPer], o[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    qf[k] = E::get(q[lane + 32 * k]);
+    qf[k] = E::get(__ldcg(q + lane + 32 * k));
     o[k] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
   const int lo = A.shape.window > 0 ? max(0, p - A.shape.window + 1) : 0;
   const int hi = min(p, A.shape.width * kPage - 1);
   for (int j = lo; j <= hi; ++j) {
-    const int pg = page_of(A.pool, e.slot, j >> 6);
+    const int pg = page_of<true>(A.pool, e.slot, j >> 6);
     if (pg < 0) continue;
     const uint8_t *kb = kv_block(A, pg, head);
     float dot = 0.f, v[kPer];
@@ -422,8 +432,8 @@ __device__ __noinline__ void row_alone(const Attend &A, const Entry &e, int head
     for (int k = 0; k < kPer; ++k) {
       const int d = lane + 32 * k;
       const int off = (d >> 6) * kBlockBytes + kv_off(j & 63, (d & 63) >> 3) + (d & 7) * 2;
-      dot = fmaf(qf[k], E::get(*reinterpret_cast<const T *>(kb + off)), dot);
-      v[k] = E::get(*reinterpret_cast<const T *>(kb + D / 64 * kBlockBytes + off));
+      dot = fmaf(qf[k], E::get(__ldcg(reinterpret_cast<const T *>(kb + off))), dot);
+      v[k] = E::get(__ldcg(reinterpret_cast<const T *>(kb + D / 64 * kBlockBytes + off)));
     }
     const float s = warp_sum(dot);
     const float nm = fmaxf(m, s), use = nm == -INFINITY ? 0.f : nm;

@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
     for (; more && ok; more = w.next(A.pool, A.batch, S, line)) {
       const int first = w.first(), count = w.count(S);
       for (int k0 = 0; k0 < count && ok; k0 += 32) {
-        const int mine = k0 + lane < count ? page_of(A.pool, w.e.slot, first + k0 + lane) : -1;
+        const int mine = k0 + lane < count ? page_of<true>(A.pool, w.e.slot, first + k0 + lane) : -1;
         for (int k = k0; k < min(count, k0 + 32); ++k, ++it) {
           const int s = it % Z::kStages;
           const uint32_t ph = static_cast<uint32_t>(it / Z::kStages) & 1u;

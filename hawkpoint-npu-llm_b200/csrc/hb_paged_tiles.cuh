@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
           int block = last ? count - 1 : (x >> 1) - 1, p0 = last ? k0 : v0, p1 = last ? k1 : v1;
           if (!is_v) {
             block = (x + 1) >> 1;
-            if ((block & 15) == 0) mine = page_of(A.pool, w.e.slot, 2 * (first + block) + lane);
+            if ((block & 15) == 0) mine = page_of<true>(A.pool, w.e.slot, 2 * (first + block) + lane);
             v0 = k0;
             v1 = k1;
             p0 = k0 = __shfl_sync(0xffffffffu, mine, 2 * (block & 15));
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         const int first = w.first(), count = w.count(S);
         bool hole = false;   // whether a page of the piece's blocks is missing
         for (int p = 2 * first + lane; p < 2 * (first + count); p += 32)
-          hole |= p * kPage < w.e.length && page_of(A.pool, w.e.slot, p) < 0;
+          hole |= p * kPage < w.e.length && page_of<true>(A.pool, w.e.slot, p) < 0;
         hole = __any_sync(0xffffffffu, hole) != 0;
         if (lane == 0) {
           info.count = count;
@@ -597,8 +597,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
           const int hi = pos - j0, lo = S.window > 0 ? hi - S.window : -1;
           bool gone[2] = {false, false};
           if (hole) {
-            gone[0] = page_of(A.pool, info.slot, 2 * (first + j)) < 0;
-            gone[1] = page_of(A.pool, info.slot, 2 * (first + j) + 1) < 0;
+            gone[0] = page_of<true>(A.pool, info.slot, 2 * (first + j)) < 0;
+            gone[1] = page_of<true>(A.pool, info.slot, 2 * (first + j) + 1) < 0;
           }
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
