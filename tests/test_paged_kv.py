@@ -652,6 +652,50 @@ def test_append_after_an_exhausted_reserve_writes_nothing():
 
 
 @gpu
+@pytest.mark.parametrize("heads", [(14, 2, 64), (32, 2, 128)])
+def test_lists_rewritten_between_calls_without_a_wait(heads):
+    """Slots, row starts and lengths that kernels of the same stream write
+    directly before each call, for calls that decode and prefill at once: the
+    same bits as when every call is waited for."""
+    torch = _torch()
+    from runtime.paged_kv import PagedKVCache
+
+    qh, kvh, d = heads
+    rows = [1, 300, 1, 77, 1, 2]
+    n, total = len(rows), sum(rows)
+    cache = PagedKVCache(1, kvh, d, 300, 12, 1500)
+    cache.pool.normal_()
+    q = torch.randn((total, qh, d), device="cuda").to(cache.dtype)
+    cache.reserve(ints(range(12)), ints([900 + 37 * i for i in range(12)]))
+    cache.status()
+    r = np.random.default_rng(3)
+    calls = []
+    for _ in range(12):
+        order = r.permutation(n)
+        calls.append((ints(r.permutation(12)[:n]), ints(np.concatenate([[0], np.cumsum(np.asarray(rows)[order])])),
+                      ints(r.integers(310, 900, 12))))
+    slots, starts = torch.empty_like(calls[0][0]), torch.empty_like(calls[0][1])
+
+    def call(x, wait):
+        slots.copy_(x[0])
+        starts.copy_(x[1])
+        cache.lengths.copy_(x[2])
+        if wait:
+            torch.cuda.synchronize()
+        out = cache.attend(0, q, slots, starts, max(rows), lse=True)
+        if wait:
+            torch.cuda.synchronize()
+        return out
+
+    want = [call(x, True) for x in calls]
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for (a, b), (c, e) in zip([call(x, False) for x in calls], want):
+            assert torch.equal(a, c) and torch.equal(b, e)
+    cache.status()
+
+
+@gpu
 @pytest.mark.parametrize("refused", ["past the table", "slot twice", "fork past the source"])
 def test_append_after_a_refused_call_writes_nothing(refused):
     """Lengths stayed as they were, so the rows' positions would be those of
