@@ -98,6 +98,10 @@ struct Shape {
     const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(r), group_inv));
     return r - q * group >= group ? q + 1 : q;
   }
+  // The first position that a row at position p sees.  Compared before it is
+  // subtracted: windows go up to 2^31 - 1, and p is negative for rows before
+  // their sequence.
+  __device__ __forceinline__ int first_seen(int p) const { return window > 0 && p >= window ? p - window + 1 : 0; }
 };
 
 struct Span {
@@ -112,7 +116,7 @@ __device__ __forceinline__ Span tile_span(const Shape &S, const Entry &e, int t)
   const int shift = S.block == 128 ? 7 : 6;
   Span s;
   s.hi = last < 0 ? 0 : min(last >> shift, (S.width * kPage - 1) >> shift) + 1;
-  s.lo = S.window > 0 ? max(0, first - S.window + 1) >> shift : 0;
+  s.lo = S.first_seen(first) >> shift;
   return s;
 }
 __device__ __forceinline__ int tile_units(const Shape &S, const Entry &e, int t) {
@@ -421,7 +425,7 @@ __device__ __noinline__ void row_alone(const Attend &A, const Entry &e, int head
     o[k] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
-  const int lo = A.shape.window > 0 ? max(0, p - A.shape.window + 1) : 0;
+  const int lo = A.shape.first_seen(p);
   const int hi = min(p, A.shape.width * kPage - 1);
   for (int j = lo; j <= hi; ++j) {
     const int pg = page_of<true>(A.pool, e.slot, j >> 6);

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
     // positions that every row of the tile sees need no mask
     const int tail = min(packed, (w.t + 1) * kRowsTile) - 1;
     const int all_hi = w.e.length - w.e.n + S.row_of(w.t * kRowsTile);
-    const int all_lo = S.window > 0 ? w.e.length - w.e.n + S.row_of(tail) - S.window + 1 : 0;
+    const int all_lo = S.first_seen(w.e.length - w.e.n + S.row_of(tail));
 
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float o[D / 8][4];
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const int j = j0 + n * 8 + (lane & 3) * 2 + (x & 1), p = pos[x >> 1];
-              if (j > p || (S.window > 0 && j <= p - S.window)) sc[n][x] = -INFINITY;
+              if (j > p || j < S.first_seen(p)) sc[n][x] = -INFINITY;
             }
         }
         uint32_t ph_[4], pl_[4];   // the weights' high and low halves

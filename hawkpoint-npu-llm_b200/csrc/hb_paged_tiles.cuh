@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
       const int pos = in ? before + i : -1;
       // positions that every row of the half sees need no mask
       const int all_hi = before + S.row_of(info.base);
-      const int all_lo = S.window > 0 ? before + S.row_of(min(info.packed, info.base + kTilesHalf) - 1) - S.window + 1 : 0;
+      const int all_lo = S.first_seen(before + S.row_of(min(info.packed, info.base + kTilesHalf) - 1));
 
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < count; ++j, ++steps) {
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         if (hole || j0 + kTilesBlock - 1 > all_hi || j0 < all_lo) {
           // sees lo < x <= hi: a bit a position, which predicates are made from
           // eight at a time (comparisons took twice the instructions)
-          const int hi = pos - j0, lo = S.window > 0 ? hi - S.window : -1;
+          const int hi = pos - j0, lo = S.first_seen(pos) - 1 - j0;
           bool gone[2] = {false, false};
           if (hole) {
             gone[0] = page_of<true>(A.pool, info.slot, 2 * (first + j)) < 0;

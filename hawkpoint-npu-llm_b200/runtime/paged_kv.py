@@ -32,6 +32,7 @@ import struct
 from runtime import hb_lib
 
 PAGE = 64
+_WIDEST = 2 ** 31 - 1   # a window's most; no context is longer
 
 # The structs of a call, filled in place: a decode step makes tens of calls, and
 # building ctypes objects for each would cost more than the launches.
@@ -210,7 +211,7 @@ class PagedKVCache:
             _, (o_row, o_head, _) = self._heads("out", out, (rows, heads))
         sums = self._empty((rows, heads), (heads, 1), dtype=self._float32, device=self.device) if lse else None
         _QUERY.pack_into(self._args_buf, 0, q.data_ptr(), q_row, q_head, out.data_ptr(), o_row, o_head,
-                         sums.data_ptr() if lse else 0, heads, window, self._scale if scale is None else scale, 0)
+                         sums.data_ptr() if lse else 0, heads, window if window < _WIDEST else _WIDEST, self._scale if scale is None else scale, 0)
         self._run(self._attend, layer, slots, row_start, rows, max_rows)
         return (out, sums) if lse else out
 

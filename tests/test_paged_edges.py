@@ -1,0 +1,22 @@
+"""Edges of the paged K/V cache operators that the cases of test_paged_kv.py leave out; the cache, the reference in
+float64 and its tolerance are that file's."""
+
+import pytest
+
+from test_paged_kv import Case, _torch
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 6, 2 ** 40])
+@pytest.mark.parametrize("heads,rows,lengths", [((14, 2, 64), [10, 3], [5, 70]), ((14, 2, 64), [300, 130], [200, 129]),
+                                                ((16, 2, 128), [40, 300], [30, 500])])
+def test_windows_wider_than_any_context(heads, rows, lengths, window):
+    """They hide nothing, also in tiles whose first rows stand before the
+    sequence (positions -5 .. -1 of the first case)."""
+    torch = _torch()
+    case = Case(heads, "bfloat16", rows, lengths, seed=41)
+    plain, plain_lse = case.check()
+    out, lse = case.check(window)
+    assert torch.equal(out, plain) and torch.equal(lse, plain_lse)
