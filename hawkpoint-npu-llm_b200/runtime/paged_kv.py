@@ -78,6 +78,8 @@ class PagedKVCache:
 
     def _bind(self, pool, table, refs, lengths):
         torch = _torch()
+        if pool.device.type != "cuda":   # the kernels would read host addresses
+            raise ValueError(f"pool on {pool.device}: must be on a CUDA device")
         elements = {torch.bfloat16: hb_lib.HB_ELEM_BF16, torch.float16: hb_lib.HB_ELEM_FP16}
         if pool.dtype not in elements:
             raise ValueError(f"pool of {pool.dtype}: must be bfloat16 or float16")

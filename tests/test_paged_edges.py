@@ -20,3 +20,16 @@ def test_windows_wider_than_any_context(heads, rows, lengths, window):
     plain, plain_lse = case.check()
     out, lse = case.check(window)
     assert torch.equal(out, plain) and torch.equal(lse, plain_lse)
+
+
+def test_a_pool_in_host_memory_is_refused():
+    """Before the library, or a device, is touched: the kernels would read host addresses."""
+    torch = _torch()
+    from runtime.paged_kv import PagedKVCache
+
+    with pytest.raises(ValueError, match="CUDA"):
+        PagedKVCache(1, 1, 64, 4, 2, 128, device="cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        PagedKVCache.wrap(torch.zeros((4, 1, 1, 2, 1, 64, 64), dtype=torch.bfloat16),
+                          torch.zeros((2, 2), dtype=torch.int32), torch.zeros(4, dtype=torch.int32),
+                          torch.zeros(2, dtype=torch.int32))
