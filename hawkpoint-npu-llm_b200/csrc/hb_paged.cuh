@@ -12,6 +12,7 @@
 
 #include <cuda_fp16.h>
 
+#include "hawkb200.h"
 #include "hb_attn.cuh"
 
 namespace hb {
@@ -50,7 +51,7 @@ struct Batch {
 };
 
 struct Entry {
-  int row0, n, length, slot;   // slot -1: none (its rows see nothing)
+  int row0, n, length, slot;   // n < 0: the row starts descend; slot -1: none (its rows see nothing)
 };
 
 // What an earlier kernel may have written.  The attention kernels read it past
@@ -65,7 +66,7 @@ template <bool PAST = false>
 __device__ __forceinline__ Entry entry_of(const Pool &P, const Batch &B, int b) {
   Entry e;
   e.row0 = min(max(read<PAST>(B.row_start + b), 0), B.rows);
-  e.n = min(max(read<PAST>(B.row_start + b + 1), e.row0), B.rows) - e.row0;
+  e.n = min(max(read<PAST>(B.row_start + b + 1), 0), B.rows) - e.row0;
   e.slot = read<PAST>(B.slots + b);
   if (e.slot < 0 || e.slot >= P.n_slots) e.slot = -1;
   e.length = e.slot < 0 ? 0 : max(read<PAST>(P.lengths + e.slot), 0);
@@ -141,15 +142,20 @@ __device__ __forceinline__ Line line_at(uint8_t *smem, int entries) {
 // Fills the line, by all threads of the block: a thread an entry, so that the
 // entries' reads are in flight together; the tiles of a long entry are
 // counted by its warp.  `take(entry)`: whether this kernel takes its rows.
+// False when row starts descend: entries would share rows, the host's bound
+// on the total would not hold, and a total that wraps leads a walk out of the
+// line.  Starts that ascend are disjoint ranges of the call's rows.
 template <class Take>
-__device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const Shape &S, const Line &line,
+__device__ __forceinline__ bool fill_line(const Pool &P, const Batch &B, const Shape &S, const Line &line,
                                           const Take &take) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  bool descends = false;
 #pragma unroll 1
   for (int b0 = warp * 32; b0 < B.entries; b0 += blockDim.x) {
     const int b = b0 + lane;
     Entry e{0, 0, 0, -1};
     if (b < B.entries) line.entry[b] = e = entry_of<true>(P, B, b);
+    descends |= e.n < 0;
     const int tiles = b < B.entries && take(e) ? tiles_of(S, e) : 0;
     int u = 0;
     if (tiles <= 4)
@@ -166,7 +172,10 @@ __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const S
     }
     if (b < B.entries) line.prefix[b + 1] = u * P.kv_heads;
   }
-  __syncthreads();
+  if (__syncthreads_or(descends)) {
+    if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(&P.control->status, HB_PAGED_BAD_INDEX);
+    return false;
+  }
   if (warp == 0) {
     int base = 0;
 #pragma unroll 1
@@ -184,6 +193,7 @@ __device__ __forceinline__ void fill_line(const Pool &P, const Batch &B, const S
     if (lane == 0) line.prefix[0] = 0;
   }
   __syncthreads();
+  return true;
 }
 
 // A walk over the tiles of one piece [u, end) of the line, the same in every
@@ -405,6 +415,21 @@ __device__ __forceinline__ int page_of(const Pool &P, int slot, int j) {
   if (slot < 0 || j < 0 || j >= P.width) return -1;
   const int pg = read<PAST>(P.table + static_cast<int64_t>(slot) * P.width + j);
   return pg >= 0 && pg < P.n_pages ? pg : -1;
+}
+
+// Rows that see nothing, [from, to) of the call, by all threads of the grid: 0
+// and -infinity.
+template <int D>
+__device__ __noinline__ void rows_unseen(const Attend &A, int from, int to) {
+  const int64_t parts = static_cast<int64_t>(A.q_heads) * (D / 8), n = static_cast<int64_t>(to - from) * parts;
+  for (int64_t x = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; x < n;
+       x += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t row = from + x / parts;
+    const int part = static_cast<int>(x % parts), head = part / (D / 8), d = part % (D / 8) * 8;
+    uint16_t *out = static_cast<uint16_t *>(A.out) + row * A.o_row + head * A.o_head + d;
+    if (A.o_vec) store8<true>(out, make_uint4(0, 0, 0, 0)); else store8<false>(out, make_uint4(0, 0, 0, 0));
+    if (A.lse != nullptr && d == 0) A.lse[row * A.q_heads + head] = -INFINITY;
+  }
 }
 
 // One output row by one warp from the positions it sees alone, in FP32.  The

@@ -25,7 +25,6 @@
 // flag, cost 1.3 us less of the host and 3.1 us more on the device.
 #pragma once
 
-#include "hawkb200.h"
 #include "hb_paged.cuh"
 
 namespace hb {

@@ -390,9 +390,10 @@ typedef struct hb_page_pool {
 
 /* The rows of a call: entry b is slot slots_dev[b] with rows row_start_dev[b]
  * .. row_start_dev[b + 1] (ascending from 0; entries + 1 values); row i of its n stands at
- * position lengths[slot] - n + i.  At most 1024 entries.  max_rows: the most
- * rows of an entry (it chooses kernels and so the rounding of weights; every
- * row is done whatever it says). */
+ * position lengths[slot] - n + i.  At most 1024 entries.  Where the starts
+ * descend attention gives 0 and -infinity for every row of the call and sets
+ * HB_PAGED_BAD_INDEX.  max_rows: the most rows of an entry (it chooses kernels
+ * and so the rounding of weights; every row is done whatever it says). */
 typedef struct hb_paged_rows {
   const int32_t *slots_dev, *row_start_dev;
   int32_t entries, rows, max_rows, reserved0;
