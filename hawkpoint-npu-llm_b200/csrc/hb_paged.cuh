@@ -417,19 +417,30 @@ __device__ __forceinline__ int page_of(const Pool &P, int slot, int j) {
   return pg >= 0 && pg < P.n_pages ? pg : -1;
 }
 
-// Rows that see nothing, [from, to) of the call, by all threads of the grid: 0
-// and -infinity.
+// The call's rows but [from, to), which see nothing, by all threads of the
+// grid: 0 and -infinity.
 template <int D>
 __device__ __noinline__ void rows_unseen(const Attend &A, int from, int to) {
-  const int64_t parts = static_cast<int64_t>(A.q_heads) * (D / 8), n = static_cast<int64_t>(to - from) * parts;
+  const int64_t parts = static_cast<int64_t>(A.q_heads) * (D / 8);
+  const int64_t n = static_cast<int64_t>(A.batch.rows - (to - from)) * parts;
   for (int64_t x = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; x < n;
        x += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = from + x / parts;
+    int64_t row = x / parts;
+    if (row >= from) row += to - from;
     const int part = static_cast<int>(x % parts), head = part / (D / 8), d = part % (D / 8) * 8;
     uint16_t *out = static_cast<uint16_t *>(A.out) + row * A.o_row + head * A.o_head + d;
     if (A.o_vec) store8<true>(out, make_uint4(0, 0, 0, 0)); else store8<false>(out, make_uint4(0, 0, 0, 0));
     if (A.lse != nullptr && d == 0) A.lse[row * A.q_heads + head] = -INFINITY;
   }
+}
+
+// The rows of a filled line's entries, all of the call's but before the first
+// and after the last.
+template <int D>
+__device__ __forceinline__ void rows_of_no_entry(const Attend &A, const Line &line) {
+  const Entry &last = line.entry[A.batch.entries - 1];
+  const int from = line.entry[0].row0, to = last.row0 + last.n;
+  if (to - from < A.batch.rows) rows_unseen<D>(A, from, to);
 }
 
 // One output row by one warp from the positions it sees alone, in FP32.  The

@@ -150,9 +150,10 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
   if (threadIdx.x < kRowsTile) s_bad[threadIdx.x] = 0;
   grid_begin();
   if (!fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group <= A.few; })) {
-    rows_unseen<D>(A, 0, A.batch.rows);
+    rows_unseen<D>(A, 0, 0);
     return;
   }
+  rows_of_no_entry<D>(A, line);
   const Cut cut(line.prefix[A.batch.entries], gridDim.x, least);
   if (static_cast<int>(blockIdx.x) >= cut.pieces) return;
   Walk w;

@@ -292,7 +292,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   // beside the rows kernel, which began when what was before it had ended
   if (!A.beside) grid_begin();
   const bool ascends = fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group > A.few; });
-  if (!ascends && A.few == 0) rows_unseen<D>(A, 0, A.batch.rows);   // else the rows kernel has done it
+  if (A.few == 0) {   // else the rows kernel does these
+    if (ascends) rows_of_no_entry<D>(A, line); else rows_unseen<D>(A, 0, 0);
+  }
   const Cut cut(ascends ? line.prefix[A.batch.entries] : 0, gridDim.x, least);
   if (static_cast<int>(blockIdx.x) >= cut.pieces) {
     asm volatile("griddepcontrol.wait;" ::: "memory");   // as at the end

@@ -17,6 +17,7 @@ A step of a serving loop, per layer the two calls in the middle::
 
 Entry b of a call is slot ``slots[b]`` with rows ``row_start[b] ..
 row_start[b + 1]``; its row i of n stands at position ``lengths[slot] - n + i``.
+Rows before the first and after the last start give 0 (and -inf).
 All index lists are int32 device tensors.  Pages are laid out
 ``[layer][kv head][K | V][head_dim / 64][64 positions][64 dims]`` with the
 16-byte blocks of a position's 64 dims stored at block ^ (position & 7);

@@ -390,7 +390,9 @@ typedef struct hb_page_pool {
 
 /* The rows of a call: entry b is slot slots_dev[b] with rows row_start_dev[b]
  * .. row_start_dev[b + 1] (ascending from 0; entries + 1 values); row i of its n stands at
- * position lengths[slot] - n + i.  At most 1024 entries.  Where the starts
+ * position lengths[slot] - n + i.  At most 1024 entries; with none a call does nothing.  Rows before the first
+ * and after the last start (room in a captured call) stand nowhere: attention
+ * gives 0 and -infinity, append q = 0 and nothing in the pages.  Where the starts
  * descend attention gives 0 and -infinity for every row of the call and sets
  * HB_PAGED_BAD_INDEX.  max_rows: the most rows of an entry (it chooses kernels
  * and so the rounding of weights; every row is done whatever it says). */

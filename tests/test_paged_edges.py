@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from runtime import hb_lib
-from test_paged_kv import Case, _torch, ints
+from test_paged_kv import Case, _torch, ints, tables
 
 gpu = pytest.mark.gpu
 
@@ -56,3 +56,31 @@ def test_row_starts_that_descend_are_refused(heads, rows):
     case.row_start = right
     out, again = case.check()
     assert torch.equal(out, good) and torch.equal(again, lse)
+
+
+@gpu
+@pytest.mark.parametrize("heads,rows", [((14, 2, 64), [1, 0, 2]), ((14, 2, 64), [1, 1, 300]), ((16, 2, 128), [200, 200, 200])])
+@pytest.mark.parametrize("before,after", [(0, 5), (3, 0), (2, 700)])
+def test_rows_of_no_entry_give_zeros(heads, rows, before, after):
+    """As a captured step with room for more rows has them; append gives q = 0 for the same rows."""
+    torch = _torch()
+    case = Case(heads, "bfloat16", rows, [250, 300, 400], seed=43)
+    want, want_lse = case.check()
+    n = case.n_rows
+    shape = (before + n + after, case.qh, case.d)
+    q = torch.randn(shape, device="cuda").to(case.dtype)
+    q[before: before + n] = case.q
+    case.q, case.row_start = q, case.row_start + before
+    wide = torch.full((shape[0], case.qh, case.d + 1), 7.0, dtype=case.dtype, device="cuda")
+    for out in (torch.full(shape, 7.0, dtype=case.dtype, device="cuda"), wide[:, :, 1:]):
+        got, lse = case.attend(out=out)
+        case.cache.status()
+        assert torch.equal(got[before: before + n], want) and torch.equal(lse[before: before + n], want_lse)
+        for part in (slice(0, before), slice(before + n, None)):
+            assert bool((got[part] == 0).all()) and bool((lse[part] == -np.inf).all())
+    assert bool((wide[:, :, 0] == 7).all())
+    cos, sin = tables(case.d, 512)
+    qkv = torch.randn((shape[0], (case.qh + 2 * case.kvh) * case.d), device="cuda").to(case.dtype)
+    turned = case.cache.append(1, qkv, case.slots, case.row_start, case.max_rows, cos, sin)
+    case.cache.status()
+    assert not bool(turned[:before].any()) and not bool(turned[before + n:].any())
