@@ -214,6 +214,7 @@ cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) 
   const bool tiles_only = !rows_only && static_cast<int64_t>(b.entries) * max_rows == b.rows;
   const size_t line = pg::line_bytes(b.entries);
   A.few = rows_only ? INT32_MAX : tiles_only ? 0 : pg::kRowsTile;
+  A.beside = !rows_only && !tiles_only ? sms : 0;
   if (!tiles_only) {
     A.shape.tile = pg::kRowsTile;
     A.shape.block = pg::kPage;
@@ -227,7 +228,6 @@ cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) 
   A.shape.extra = pg::kTilesExtra;
   A.arrived = A.arrived2;
   A.parts = A.parts2;
-  A.beside = !tiles_only;   // the rows kernel's blocks leave first; it reads nothing of that one's
   return launch(pg::paged_tiles_kernel<D, T>, sms, pg::kTilesThreads, pg::TilesSize<D>::kSmem + line, st, A, pg::kTilesLeast);
 }
 

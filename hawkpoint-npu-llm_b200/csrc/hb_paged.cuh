@@ -30,7 +30,8 @@ struct Control {
   int status;    // HB_PAGED_* bits, cleared by hb_paged_status
   int copies;    // entries of the copy list
   int refused;   // a reserve or fork changed nothing since the status was read
-  int pad[5];
+  int began;     // pair_arrive, zero between calls
+  int pad[4];
 };
 static_assert(sizeof(Control) == 64, "control block");
 
@@ -55,7 +56,7 @@ struct Entry {
 };
 
 // What an earlier kernel may have written.  The attention kernels read it past
-// L1 (PAST): the tiles kernel beside a rows kernel begins without a wait of its own.
+// L1 (PAST): a block needs each once.
 template <bool PAST, class T>
 __device__ __forceinline__ T read(const T *p) {
   return PAST ? __ldcg(p) : *p;
@@ -76,11 +77,43 @@ __device__ __forceinline__ Entry entry_of(const Pool &P, const Batch &B, int b) 
 // Every kernel here is launched early (programmatic launch): its blocks take
 // their places while the kernel before it ends, wait for it and what it wrote,
 // and let the next one do the same.  Waiting comes first, so that at most two
-// kernels of a stream are under way.
+// kernels of a stream are under way (three where an attention call has two).
 __device__ __forceinline__ void grid_begin() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+
+// A call of two kernels, the second launched early and beside the first, whose
+// results it does not need, only what the first one's wait made visible.  A
+// wait of its own would last until the first one ends (7 to 12 us more in a
+// step of 96 streams of which 12 or 24 have chunks).  So the first's first block
+// counts kFirst up when it has waited, before it lets the second begin, and
+// the second's blocks count one up each: a block that finds the first one's
+// count has what came before it (release and acquire, cumulative), one that
+// does not (it cannot happen, but nothing here depends on that) waits in full.
+// Whoever completes the count sets it to zero.  True: kFirst was there.
+constexpr int kFirst = 1 << 16;   // more than the second kernel has blocks
+__device__ __forceinline__ bool pair_arrive(Control *c, int n, int blocks) {
+  int old;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], %2;" : "=r"(old) : "l"(&c->began), "r"(n) : "memory");
+  if (old + n == kFirst + blocks) atomicExch(&c->began, 0);
+  return old >= kFirst;
+}
+__device__ __forceinline__ void first_begin(Control *c, int blocks) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (blockIdx.x == 0 && threadIdx.x == 0) pair_arrive(c, kFirst, blocks);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+// `seen`: a word of shared memory.  The second kernel lets none begin early,
+// and waits for the first one before it ends (grid_end), so that whoever waits
+// for it has waited for both.
+__device__ __forceinline__ void second_begin(Control *c, int *seen) {
+  if (threadIdx.x == 0) *seen = pair_arrive(c, 1, gridDim.x);
+  __syncthreads();
+  if (*seen == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("fence.proxy.async;" ::: "memory");   // the bulk copies of pages, which earlier kernels wrote
+}
+__device__ __forceinline__ void grid_end() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---- division of an attention call --------------------------------------------
 // The rows of an entry and the q heads of a kv head's group are packed into
@@ -396,7 +429,7 @@ struct Attend {
   float scale, scale_log2;         // of the scores; times log2(e)
   int q_vec, o_vec;                // q rows / out rows are 16-byte aligned
   int o_wide;                      // 32-byte aligned
-  int beside;                      // the tiles kernel runs beside the rows kernel of the same call
+  int beside;                      // blocks of the tiles kernel that runs beside the rows kernel, 0: one has all entries
   int few;                         // entries of up to this many packed rows are the rows kernel's, others the tiles'
   float *parts;                    // joined tiles: per piece two parts
   int *arrived;                    // per piece, zero between launches

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
     fence_mbar_init();
   }
   if (threadIdx.x < kRowsTile) s_bad[threadIdx.x] = 0;
-  grid_begin();
+  if (A.beside) first_begin(A.pool.control, A.beside); else grid_begin();
   if (!fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group <= A.few; })) {
     rows_unseen<D>(A, 0, 0);
     return;

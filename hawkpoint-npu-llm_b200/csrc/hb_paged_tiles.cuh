@@ -289,15 +289,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     mbar_init(&bars.done, 1);
     fence_mbar_init();
   }
-  // beside the rows kernel, which began when what was before it had ended
-  if (!A.beside) grid_begin();
+  if (A.beside) second_begin(A.pool.control, s_seen); else grid_begin();
   const bool ascends = fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group > A.few; });
   if (A.few == 0) {   // else the rows kernel does these
     if (ascends) rows_of_no_entry<D>(A, line); else rows_unseen<D>(A, 0, 0);
   }
   const Cut cut(ascends ? line.prefix[A.batch.entries] : 0, gridDim.x, least);
   if (static_cast<int>(blockIdx.x) >= cut.pieces) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // as at the end
+    grid_end();
     return;
   }
   if (warp == 0) t_alloc(&s_tmem, 512);
@@ -836,9 +835,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   __syncthreads();
   t_after();
   if (warp == 0) t_dealloc(s_tmem, 512);
-  // launched beside the rows kernel of the same call, this one is not done
-  // before that one
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_end();
 }
 
 }  // namespace paged

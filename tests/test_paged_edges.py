@@ -84,3 +84,60 @@ def test_rows_of_no_entry_give_zeros(heads, rows, before, after):
     turned = case.cache.append(1, qkv, case.slots, case.row_start, case.max_rows, cos, sin)
     case.cache.status()
     assert not bool(turned[:before].any()) and not bool(turned[before + n:].any())
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(14, 2, 64), (32, 2, 128)])
+def test_mixed_steps_back_to_back(heads):
+    """Steps that decode and prefill at once, each layer's append directly
+    before its attention, nothing waited for: the same bits as when every
+    call is waited for."""
+    torch = _torch()
+    from runtime.paged_kv import PagedKVCache
+
+    qh, kvh, d = heads
+    rows = [1, 260, 1, 90, 1]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    qkv = torch.randn((12, sum(rows), (qh + 2 * kvh) * d), device="cuda", generator=g).bfloat16()
+    cos, sin = tables(d, 4096)
+    slots, start, counts = ints([3, 0, 4, 1, 2]), ints(np.concatenate([[0], np.cumsum(rows)])), ints(rows)
+
+    def steps(wait):
+        cache, outs = PagedKVCache(2, kvh, d, 120, 5, 2048), []
+        q = torch.empty((sum(rows), qh, d), dtype=torch.bfloat16, device="cuda")
+        for i in range(0, 12, 2):
+            cache.reserve(slots, counts)
+            for layer in range(2):
+                cache.append(layer, qkv[i + layer], slots, start, max(rows), cos, sin, out=q)
+                if wait:
+                    torch.cuda.synchronize()
+                outs.append(cache.attend(layer, q, slots, start, max(rows), lse=True))
+                if wait:
+                    torch.cuda.synchronize()
+        cache.status()
+        return outs
+
+    want = steps(True)
+    for _ in range(3):
+        for (a, b), (c, e) in zip(steps(False), want):
+            assert torch.equal(a, c) and torch.equal(b, e)
+    # and captured, replayed back to back
+    cache = PagedKVCache(1, kvh, d, 120, 5, 2048)
+    cache.reserve(slots, counts)
+
+    def layer():
+        return cache.attend(0, cache.append(0, qkv[0], slots, start, max(rows), cos, sin), slots, start, max(rows), lse=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = layer()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [layer() for _ in range(3)]
+    for _ in range(20):
+        graph.replay()
+    cache.status()
+    assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got)
