@@ -139,8 +139,9 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
       if (!is_v) {
         if (pos >= 0) {
           const int64_t off = static_cast<int64_t>(pos) * (D / 2) + c * 8;
-          const float4 c0 = __ldg(reinterpret_cast<const float4 *>(A.cos + off)), c1 = __ldg(reinterpret_cast<const float4 *>(A.cos + off) + 1);
-          const float4 s0 = __ldg(reinterpret_cast<const float4 *>(A.sin + off)), s1 = __ldg(reinterpret_cast<const float4 *>(A.sin + off) + 1);
+          // plain loads, as load8's: the heads of a row share them in L1
+          const float4 c0 = *reinterpret_cast<const float4 *>(A.cos + off), c1 = *(reinterpret_cast<const float4 *>(A.cos + off) + 1);
+          const float4 s0 = *reinterpret_cast<const float4 *>(A.sin + off), s1 = *(reinterpret_cast<const float4 *>(A.sin + off) + 1);
           const float cv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
           const float sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
           rope8<T>(a, b, cv, sv, a, b);

@@ -141,3 +141,49 @@ def test_mixed_steps_back_to_back(heads):
         graph.replay()
     cache.status()
     assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got)
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(14, 2, 64), (32, 2, 128)])
+def test_q_and_rope_tables_rewritten_between_calls_without_a_wait(heads):
+    """The kernel before writes the tables that append turns by, append the q
+    that attention reads, in the same memory each time."""
+    torch = _torch()
+    from runtime.paged_kv import PagedKVCache
+
+    qh, kvh, d = heads
+    n = 40
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    new = torch.randn((8, n, (qh + 2 * kvh) * d), device="cuda", generator=g).bfloat16()
+    some = [tables(d, 1024)]
+    for _ in range(7):
+        some.append(tuple(t.roll(17, 0) for t in some[-1]))
+    slots, start, ones = ints(range(n)), ints(range(n + 1)), ints([1] * n)
+
+    def steps(wait):
+        cache, outs = PagedKVCache(1, kvh, d, n * 8, n, 512), []
+        cache.pool.fill_(0.5)
+        cache.reserve(slots, ints([300 + i for i in range(n)]))
+        q = torch.empty((n, qh, d), dtype=torch.bfloat16, device="cuda")
+        qkv, cos, sin = torch.empty_like(new[0]), torch.empty_like(some[0][0]), torch.empty_like(some[0][1])
+        for x, (c, s) in zip(new, some):
+            cache.reserve(slots, ones)
+            qkv.copy_(x)
+            cos.copy_(c)
+            sin.copy_(s)
+            if wait:
+                torch.cuda.synchronize()
+            cache.append(0, qkv, slots, start, 1, cos, sin, out=q)
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(cache.attend(0, q, slots, start, 1, lse=True))
+            if wait:
+                torch.cuda.synchronize()
+        cache.status()
+        return outs
+
+    want = steps(True)
+    for _ in range(3):
+        for (a, b), (c, e) in zip(steps(False), want):
+            assert torch.equal(a, c) and torch.equal(b, e)
