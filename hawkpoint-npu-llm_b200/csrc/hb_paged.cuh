@@ -358,6 +358,7 @@ template <class T>
 struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
+  static constexpr uint32_t kInfinity = 0x7f80;
   static __device__ __forceinline__ float lo(uint32_t u) { return bf_lo(u); }
   static __device__ __forceinline__ float hi(uint32_t u) { return bf_hi(u); }
   static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -370,6 +371,7 @@ struct Elem<__nv_bfloat16> {
 };
 template <>
 struct Elem<__half> {
+  static constexpr uint32_t kInfinity = 0x7c00;
   static __device__ __forceinline__ float lo(uint32_t u) { return __half2float(__ushort_as_half(u & 0xffffu)); }
   static __device__ __forceinline__ float hi(uint32_t u) { return __half2float(__ushort_as_half(u >> 16)); }
   static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
@@ -476,49 +478,150 @@ __device__ __forceinline__ void rows_of_no_entry(const Attend &A, const Line &li
   if (to - from < A.batch.rows) rows_unseen<D>(A, from, to);
 }
 
-// One output row by one warp from the positions it sees alone, in FP32.  The
-// tiled kernels multiply hidden positions by weight zero, which an infinity or
-// NaN among their V would turn into NaN; a row that comes out not finite is
-// done again here, so that what a row does not see never reaches it.
+// ---- rows that did not come out finite ------------------------------------------
+// The tiled kernels multiply the V of positions that a row does not see by
+// weight zero, and infinity or NaN among them makes that NaN; the rows kernel
+// multiplies V by two halves of a weight, which makes an infinity NaN.  So a
+// row whose sum of weights is finite and whose output is not is looked at
+// again, by its warp, after the block's last tile: no wait with a limit is
+// open then, however long that takes.  A row whose sum is not finite saw the
+// NaN itself (scores are masked, so nothing hidden gets there): it is NaN.
+
+// Positions of [from, to) whose V holds an infinity or NaN.
+struct Odd {
+  int first, last;   // of either; last < first: none
+  bool infinity;
+};
 template <int D, class T>
-__device__ __noinline__ void row_alone(const Attend &A, const Entry &e, int head, int i, int g) {
-  using E = Elem<T>;
-  constexpr int kPer = D / 32;
+__device__ __forceinline__ Odd odd_values(const Attend &A, const Entry &e, int head, int from, int to) {
+  constexpr uint32_t kInf = Elem<T>::kInfinity;
   const int lane = threadIdx.x & 31;
-  const int qh = head * A.shape.group + g, row = e.row0 + i, p = e.length - e.n + i;
-  const T *q = static_cast<const T *>(A.q) + row * A.q_row + qh * A.q_head;
-  float qf[kPer], o[kPer];
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    qf[k] = E::get(__ldcg(q + lane + 32 * k));
-    o[k] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  const int lo = A.shape.first_seen(p);
-  const int hi = min(p, A.shape.width * kPage - 1);
-  for (int j = lo; j <= hi; ++j) {
+  int first = INT32_MAX, last = -1;
+  bool infinity = false;
+  to = min(to, e.length);
+  for (int j = from + lane; j < to; j += 32) {
     const int pg = page_of<true>(A.pool, e.slot, j >> 6);
     if (pg < 0) continue;
-    const uint8_t *kb = kv_block(A, pg, head);
-    float dot = 0.f, v[kPer];
+    const uint8_t *vb = kv_block(A, pg, head) + D / 64 * kBlockBytes;
+    bool odd = false;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int d = lane + 32 * k;
-      const int off = (d >> 6) * kBlockBytes + kv_off(j & 63, (d & 63) >> 3) + (d & 7) * 2;
-      dot = fmaf(qf[k], E::get(__ldcg(reinterpret_cast<const T *>(kb + off))), dot);
-      v[k] = E::get(__ldcg(reinterpret_cast<const T *>(kb + D / 64 * kBlockBytes + off)));
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(vb + (c >> 3) * kBlockBytes + kv_off(j & 63, c & 7)));
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t lo = u[x] & 0x7fffu, hi = u[x] >> 16 & 0x7fffu;
+        odd |= lo >= kInf || hi >= kInf;
+        infinity |= lo == kInf || hi == kInf;
+      }
     }
-    const float s = warp_sum(dot);
-    const float nm = fmaxf(m, s), use = nm == -INFINITY ? 0.f : nm;
+    if (odd) {
+      first = min(first, j);
+      last = j;
+    }
+  }
+  return Odd{__reduce_min_sync(0xffffffffu, first), __reduce_max_sync(0xffffffffu, last),
+             __any_sync(0xffffffffu, infinity) != 0};
+}
+
+// One output row by one warp from the positions it sees alone, in FP32: 32 of
+// them a step, a score a lane, the newest first (a row that is NaN by its own
+// K or V ends there).
+template <int D, class T>
+__device__ __forceinline__ void row_alone(const Attend &A, const Entry &e, int head, int i, int g) {
+  using E = Elem<T>;
+  const int lane = threadIdx.x & 31;
+  const int qh = head * A.shape.group + g, row = e.row0 + i, p = e.length - e.n + i;
+  const uint16_t *q = static_cast<const uint16_t *>(A.q) + row * A.q_row + qh * A.q_head;
+  const int lo = A.shape.first_seen(p);
+  float m = -INFINITY, l = 0.f, o[D / 32];   // l: this lane's part; dims 64 k + 2 lane, 64 k + 2 lane + 1
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
+  bool nan = false;
+  for (int top = min(p, A.shape.width * kPage - 1); top >= lo && !nan; top -= 32) {
+    const int j = top - lane, pg = j >= lo ? page_of<true>(A.pool, e.slot, j >> 6) : -1;
+    float s = -INFINITY;
+    if (pg >= 0) {
+      const uint8_t *kb = kv_block(A, pg, head);
+      s = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 k = __ldcg(reinterpret_cast<const uint4 *>(kb + (c >> 3) * kBlockBytes + kv_off(j & 63, c & 7)));
+        const uint4 x = load8<false>(q + c * 8);
+        const uint32_t a[4] = {k.x, k.y, k.z, k.w}, b[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) s = fmaf(E::lo(a[y]), E::lo(b[y]), fmaf(E::hi(a[y]), E::hi(b[y]), s));
+      }
+    }
+    float mx = s;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+    nan = __any_sync(0xffffffffu, !(s < INFINITY)) != 0;   // NaN, or infinity less infinity
+    const float nm = fmaxf(m, mx), use = nm == -INFINITY ? 0.f : nm;
     const float a = exp2_approx((m - use) * A.scale_log2), w = exp2_approx((s - use) * A.scale_log2);
     m = nm;
     l = fmaf(l, a, w);
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) o[k] = fmaf(w, v[k], o[k] * a);
-  }
-  T *out = static_cast<T *>(A.out) + row * A.o_row + qh * A.o_head;
+    for (int k = 0; k < D / 32; ++k) o[k] *= a;
+#pragma unroll 8
+    for (int x = 0; x < 32; ++x) {
+      const int px = __shfl_sync(0xffffffffu, pg, x);
+      const float wx = __shfl_sync(0xffffffffu, w, x);
+      if (px < 0) continue;
+      const uint8_t *vb = kv_block(A, px, head) + D / 64 * kBlockBytes + kv_off((top - x) & 63, lane >> 2) + (lane & 3) * 4;
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) out[lane + 32 * k] = E::put(l == 0.f ? 0.f : o[k] / l);
+      for (int k = 0; k < D / 64; ++k) {
+        const uint32_t v = __ldcg(reinterpret_cast<const uint32_t *>(vb + k * kBlockBytes));
+        o[2 * k] = fmaf(wx, E::lo(v), o[2 * k]);
+        o[2 * k + 1] = fmaf(wx, E::hi(v), o[2 * k + 1]);
+      }
+    }
+    bool gone = true;   // every dim is NaN, and stays it
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) gone &= o[k] != o[k];
+    nan |= __all_sync(0xffffffffu, gone) && __any_sync(0xffffffffu, l > 0.f);
+  }
+  l = warp_sum(l);
+  T *out = static_cast<T *>(A.out) + row * A.o_row + qh * A.o_head + 2 * lane;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k)
+    out[(k >> 1) * 64 + (k & 1)] = E::put(nan ? NAN : l == 0.f ? 0.f : o[k] / l);
+}
+
+// A warp's rows, `first` .. first + count - 1 of each tile of the block's piece,
+// that are not finite.  done: bit 0 and bit 1 say that this block finished the
+// cut tile that it entered and the one that it opened.  (The line is cut again:
+// the kernels' loops have no registers to keep that for this.)
+template <int D, class T>
+__device__ __noinline__ void rows_again(const Attend &A, const Line line, int least, int first, int count,
+                                        unsigned done) {
+  const Shape &S = A.shape;
+  const int lane = threadIdx.x & 31;
+  const Cut cut(line.prefix[A.batch.entries], gridDim.x, least);
+  Walk w;
+  w.u = cut.begin(blockIdx.x);
+  w.end = cut.begin(blockIdx.x + 1);
+  __syncwarp();   // its lanes' stores of the rows
+  for (bool more = w.start(A.pool, A.batch, S, line); more; more = w.next(A.pool, A.batch, S, line)) {
+    if (!w.whole() && !(done >> (w.opens() ? 1 : 0) & 1u)) continue;
+    Odd odd{0, -1, false};
+    bool known = false;
+    const int base = w.t * S.tile + first, end = min(w.e.n * S.group, base + count);
+    for (int r = base; r < end; ++r) {
+      const int i = S.row_of(r), g = r - i * S.group, p = w.e.length - w.e.n + i;
+      const uint16_t *out =
+          static_cast<const uint16_t *>(A.out) + (w.e.row0 + i) * A.o_row + (w.head * S.group + g) * A.o_head + lane;
+      bool bad = false;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) bad |= (__ldcg(out + 32 * k) & 0x7fffu) >= Elem<T>::kInfinity;
+      if (!__any_sync(0xffffffffu, bad)) continue;
+      if (!known) odd = odd_values<D, T>(A, w.e, w.head, w.span.lo * S.block, w.span.hi * S.block);
+      known = true;
+      // NaN that the row sees, and nothing else in its tile: it stays
+      const bool stays = odd.first <= odd.last && !odd.infinity && odd.first >= S.first_seen(p) && odd.last <= p;
+      if (!stays) row_alone<D, T>(A, w.e, w.head, i, g);
+    }
+  }
 }
 
 }  // namespace paged

@@ -96,7 +96,7 @@ __device__ __forceinline__ uint32_t q_pair(const Attend &A, const T *row, int co
 }
 
 // Row r's kPer values v[] (dims d0 ..) of a finished tile, and its lse by the
-// thread that holds dim 0.  False when a value is not finite.
+// thread that holds dim 0.  False when a value is not finite though l is.
 template <int D, class T, int kPer>
 __device__ __forceinline__ bool store_row(const Attend &A, const Entry &e, int head, int r, int d0, const float *o,
                                           float m, float l) {
@@ -123,7 +123,7 @@ __device__ __forceinline__ bool store_row(const Attend &A, const Entry &e, int h
     for (int k = 0; k < kPer; ++k) out[k] = E::put(v[k]);
   }
   if (A.lse != nullptr && d0 == 0) A.lse[row * A.q_heads + qh] = l == 0.f ? -INFINITY : m * A.scale + logf(l);
-  return fine;
+  return fine || !(l <= 3.4e38f);
 }
 
 // Two blocks a multiprocessor with heads of 64 (three would have to keep parts
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
   __shared__ __align__(8) uint64_t s_full[Z::kStages], s_empty[Z::kStages];
   __shared__ int s_valid[Z::kStages];
   __shared__ float s_m[kRowsWarps][kRowsTile], s_l[kRowsWarps][kRowsTile];
-  __shared__ int s_bad[kRowsTile], s_last;
+  __shared__ int s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Shape S = A.shape;
   const Line line = line_at(smem + Z::kSmem, A.batch.entries);
@@ -149,7 +149,6 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
     }
     fence_mbar_init();
   }
-  if (threadIdx.x < kRowsTile) s_bad[threadIdx.x] = 0;
   if (A.beside) first_begin(A.pool.control, A.beside); else grid_begin();
   if (!fill_line(A.pool, A.batch, S, line, [&](const Entry &e) { return e.n * S.group <= A.few; })) {
     rows_unseen<D>(A, 0, 0);
@@ -214,6 +213,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
   float *join = reinterpret_cast<float *>(smem + Z::kStages * Z::kStageBytes);
   const int mat = lane >> 3, mrow = lane & 7;
   bool ok = true;
+  unsigned done = 0;   // of rows_again; bit 2: there is a row to look at
   for (; more; more = w.next(A.pool, A.batch, S, line)) {
     const int packed = w.e.n * S.group;
     // this thread's rows of the tile: r, r + 8
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
       __syncwarp();
       if (lane == 0) mbar_arrive_count(&s_empty[s], 1);
     }
-    if (rows_any(!ok)) break;   // a wait gave up: the control block says which
+    if (rows_any(!ok)) return;   // a wait gave up: the control block says which
 
     // join the warps' halves of the tile
 #pragma unroll
@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
       rows_sync();
       write = write && s_last != 0;
       if (s_last != 0) {
+        done |= w.opens() ? 2u : 1u;
         // part k: the second slot of the first piece, the first of the others
         const float *base = A.parts + static_cast<int64_t>(c0) * 2 * Z::kPartFloats;
         auto part_at = [&](int k) { return base + (static_cast<int64_t>(k) * 2 + (k == 0 ? 1 : 0)) * Z::kPartFloats; };
@@ -425,19 +426,9 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) paged_rows_kern
         }
       }
     }
-    const bool bad = write && !store_row<D, T, kPer>(A, w.e, w.head, row, d0, v, tm, tl);
-    if (bad) s_bad[r] = 1;
-    if (rows_any(bad)) {   // rows with infinities or NaN: each again, alone
-      for (int x = warp; x < kRowsTile; x += kRowsWarps)
-        if (s_bad[x]) {
-          const int y = w.t * kRowsTile + x;
-          row_alone<D, T>(A, w.e, w.head, y / S.group, y % S.group);
-        }
-      rows_sync();
-      if (threadIdx.x < kRowsTile) s_bad[threadIdx.x] = 0;
-      rows_sync();
-    }
+    if (write && !store_row<D, T, kPer>(A, w.e, w.head, row, d0, v, tm, tl)) done |= 4u;
   }
+  if (__any_sync(0xffffffffu, done & 4u)) rows_again<D, T>(A, line, least, warp * (kRowsTile / kRowsWarps), kRowsTile / kRowsWarps, done);
 }
 
 }  // namespace paged

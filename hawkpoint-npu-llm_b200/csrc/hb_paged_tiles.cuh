@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   __shared__ uint32_t s_tmem;
   __shared__ TileInfo s_info[2][kInfoSlots];
   __shared__ int s_last[2], s_seen[2];
+  __shared__ unsigned s_done[8];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *ring = smem + 2 * Z::kQ * Z::kOperand;   // behind the q of either half, kQ tiles
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -554,6 +555,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
     uint32_t steps = 0, n_tiles = 0;   // of this half so far
     uint32_t turns = 0;                // steps of tiles with two halves
     bool ok = true;
+    unsigned &done = s_done[warp];     // of rows_again; bit 2: there is a row to look at.  Not in a register
+    if (lane == 0) done = 0;
     auto wait = [&](uint64_t *bar, uint32_t phase) {
       ok = __all_sync(0xffffffffu, ok && t_wait(bar, phase & 1u, ctrl, A.limit_ns, kWhereFull)) != 0;
       return ok;
@@ -725,7 +728,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
           }
           s_seen[h] = seen;
         }
-        if (!half_sync() || s_seen[h] == 0) break;
+        if (!half_sync()) break;
+        ok = s_seen[h] != 0;
+        if (!ok) break;
+        if (lane == 0) done |= info.opens ? 2u : 1u;
         const float *p = A.parts + h * Z::kPartFloats + 128 * D + r;
         const float om = m, ol = l;
         m = -INFINITY;
@@ -815,17 +821,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
         }
       }
       t_before();   // this half's O is read: its next p arrival says so
-      // rows with infinities or NaN: each again, alone, by its own warp
       float w0, w1;
       f2_split(wrong, w0, w1);
-      unsigned again = __ballot_sync(0xffffffffu, w0 + w1 != 0.f);
-      while (again) {
-        const int x = __ffs(again) - 1;
-        again &= again - 1;
-        const int y = info.base + (warp & 3) * 32 + x, yi = S.row_of(y);
-        __syncwarp();
-        row_alone<D, T>(A, Entry{info.row0, info.n, info.length, info.slot}, info.head, yi, y - yi * S.group);
-      }
+      if (__any_sync(0xffffffffu, w0 + w1 != 0.f && l <= 3.4e38f) && lane == 0) done |= 4u;
     }
   }
   __syncwarp();
@@ -835,6 +833,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) paged_tiles_kernel(const __g
   __syncthreads();
   t_after();
   if (warp == 0) t_dealloc(s_tmem, 512);
+  // here, not in the softmax branch: a call there costs its loops registers (whole prompts 170 us instead of 165)
+  if (warp < 8 && s_done[warp] & 4u)
+    rows_again<D, T>(A, line_at(smem + (2 * Z::kQ + Z::kStages) * Z::kOperand, A.batch.entries), least, warp * 32, 32,
+                     s_done[warp]);
   grid_end();
 }
 

@@ -432,8 +432,8 @@ int hb_paged_status(const hb_page_pool *pool, int32_t *status, void *stream);
 /* out = softmax(scale q.K + mask) V over one layer's pages: a row sees the
  * mapped positions up to its own, with a window the last `window` of them.  A
  * row that sees none gives zeros and an lse of -infinity.  Positions that a row does
- * not see never reach it, whatever they hold (a row that meets infinities or
- * NaN is done once more, slowly).  Scores, sums and the running maximum are
+ * not see never reach it, whatever they hold (rows near infinities or NaN in V
+ * are done once more, slowly; a row that sees a NaN score is NaN at once).  Scores, sums and the running maximum are
  * FP32; for the product with V the weights are rounded to the element type in
  * calls with long chunks, else kept to twice its bits; out is rounded once.
  * out must not overlap q. */

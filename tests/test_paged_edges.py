@@ -187,3 +187,87 @@ def test_q_and_rope_tables_rewritten_between_calls_without_a_wait(heads):
     for _ in range(3):
         for (a, b), (c, e) in zip(steps(False), want):
             assert torch.equal(a, c) and torch.equal(b, e)
+
+
+def poisoned(case, position, kind, value, dim=None):
+    """Sets a position's K (0) or V (1) of the first entry, all dims of it or one."""
+    page = case.cache.pool[int(case.table_np[case.slots_np[0], position // 64]), 1, :, kind, :, position % 64]
+    if dim is None:
+        page[:] = value
+    else:  # 16-byte blocks lie at block ^ (position & 7)
+        page[:, dim // 64, (dim % 64 // 8 ^ position % 8) * 8 + dim % 8] = value
+
+
+def timed(call):
+    torch = _torch()
+    call()
+    best = 1e9
+    for _ in range(3):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        call()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+@gpu
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("heads,rows,lengths", [((14, 2, 64), [1500], [1500]), ((16, 2, 128), [700], [900]),
+                                                ((14, 2, 64), [1] * 8, [3000] * 8)])
+def test_a_nan_that_rows_see_is_not_looked_for_again(heads, rows, lengths, kind):
+    """Rows that see it are NaN from the first pass on; only rows that it is
+    hidden from are done again."""
+    torch = _torch()
+    case = Case(heads, "bfloat16", rows, lengths, seed=44)
+    clean, clean_lse = case.check()
+    fast = timed(case.attend)
+    poisoned(case, 3, kind, float("nan"))
+    out, lse = case.attend()
+    slow = timed(case.attend)
+    case.cache.status()
+    sees = torch.arange(lengths[0] - rows[0], lengths[0], device="cuda") >= 3
+    n = rows[0]
+    assert bool(torch.isnan(out[:n][sees]).all()) and bool(torch.isfinite(out[:n][~sees]).all())
+    assert torch.equal(torch.isnan(lse[:n]), (sees & (kind == 0))[:, None].expand(n, case.qh))
+    _, _, tol, _ = case.reference()
+    assert bool(((out[:n][~sees].double() - clean[:n][~sees].double()).abs() <= 2 * tol[:n][~sees]).all())
+    assert torch.equal(out[n:], clean[n:]) and torch.equal(lse[n:], clean_lse[n:])
+    assert slow < 10 * fast + 0.5  # ms; a second pass over every row took hundreds of times as long
+
+
+@gpu
+def test_an_infinity_in_one_dim_of_v_stays_there():
+    torch = _torch()
+    case = Case((14, 2, 64), "bfloat16", [200, 5], [300, 90], seed=45)
+    clean, lse = case.check()
+    poisoned(case, 150, 1, float("inf"), dim=37)
+    out, same = case.attend()
+    case.cache.status()
+    sees = torch.arange(100, 300, device="cuda") >= 150
+    assert bool((out[:200][sees][:, :, 37] == np.inf).all()) and torch.equal(lse, same)
+    out[:200, :, 37] = torch.where(sees[:, None], 0, out[:200, :, 37])
+    clean[:200, :, 37] = torch.where(sees[:, None], 0, clean[:200, :, 37])
+    _, _, tol, _ = case.reference()
+    assert bool(((out.double() - clean.double()).abs() <= 2 * tol).all())
+
+
+@gpu
+@pytest.mark.parametrize("rows", [300, 1])
+@pytest.mark.parametrize("where", ["K seen", "V seen", "hidden"])
+def test_a_nan_in_a_long_context_leaves_the_status_clean(rows, where):
+    """Rows are done again after the pipeline's last wait, not between waits
+    with a limit."""
+    torch = _torch()
+    length = 160_000
+    case = Case((4, 1, 64), "bfloat16", [rows, 1], [length, 64], seed=46)
+    clean, _ = case.check()
+    _, _, tol, _ = case.reference()
+    poisoned(case, length - 1 if where == "hidden" else 5, 0 if where == "K seen" else 1, float("nan"))
+    out, lse = case.attend()
+    case.cache.status()
+    nan = slice(rows - 1, rows) if where == "hidden" else slice(0, rows)
+    assert bool(torch.isnan(out[nan]).all())
+    fine = [i for i in range(rows + 1) if not nan.start <= i < nan.stop]
+    assert bool(((out[fine].double() - clean[fine].double()).abs() <= 2 * tol[fine]).all())
