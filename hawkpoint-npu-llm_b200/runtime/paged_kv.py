@@ -145,6 +145,8 @@ class PagedKVCache:
 
     def _run(self, fn, layer, slots, row_start, rows, max_rows):
         entries = slots.numel()
+        if not 0 <= layer < self.layers:   # ctypes would cut it to 32 bits
+            raise ValueError(f"layer {layer} outside [0, {self.layers})")
         if max_rows < 0 or (entries == 0 and rows > 0):
             raise ValueError("max_rows must not be negative, and rows need an entry")
         _ROWS.pack_into(self._rows_buf, 0, self._list("slots", slots), self._list("row_start", row_start, entries + 1),

@@ -271,3 +271,17 @@ def test_a_nan_in_a_long_context_leaves_the_status_clean(rows, where):
     assert bool(torch.isnan(out[nan]).all())
     fine = [i for i in range(rows + 1) if not nan.start <= i < nan.stop]
     assert bool(((out[fine].double() - clean[fine].double()).abs() <= 2 * tol[fine]).all())
+
+
+@gpu
+def test_layers_past_32_bits_are_refused():
+    """2^32 + 1 is not layer 1."""
+    torch = _torch()
+    case = Case((4, 2, 64), "bfloat16", [1, 2], [5, 9], seed=47)
+    cos, sin = tables(64, 64)
+    qkv = torch.zeros((3, 8 * 64), dtype=torch.bfloat16, device="cuda")
+    for layer in (2 ** 32 + 1, 2 ** 32, -2 ** 32, 2 ** 70):
+        with pytest.raises(ValueError):
+            case.cache.attend(layer, case.q, case.slots, case.row_start, 2)
+        with pytest.raises(ValueError):
+            case.cache.append(layer, qkv, case.slots, case.row_start, 2, cos, sin)
