@@ -268,6 +268,8 @@ class PagedKVCache:
         torch = _torch()
         length = int(self.lengths[slot])
         pages = self.table[slot, : -(-length // PAGE)].long()
+        if len(pages) * PAGE < length or bool(((pages < 0) | (pages >= self.pool.shape[0])).any()):
+            raise ValueError(f"slot {slot} has no page for some of its {length} positions")
         x = self.pool[pages, layer].view(len(pages), self.kv_heads, 2, -1, PAGE, 8, 8)
         at = torch.arange(PAGE, device=self.device)[:, None]
         x = x[..., at, torch.arange(8, device=self.device)[None, :] ^ (at & 7), :]

@@ -285,3 +285,18 @@ def test_layers_past_32_bits_are_refused():
             case.cache.attend(layer, case.q, case.slots, case.row_start, 2)
         with pytest.raises(ValueError):
             case.cache.append(layer, qkv, case.slots, case.row_start, 2, cos, sin)
+
+
+@gpu
+def test_rows_of_missing_pages_are_refused():
+    """rows() has no page to read there, and reads no other one's."""
+    case = Case((4, 2, 64), "bfloat16", [1, 1], [200, 9], seed=48)
+    slot = int(case.slots_np[0])
+    assert case.cache.rows(1, slot).shape == (2, 2, 200, 64)
+    for bad in (-1, 10 ** 6):
+        case.cache.table[slot, 1] = bad
+        with pytest.raises(ValueError):
+            case.cache.rows(1, slot)
+    case.cache.lengths[slot] = 10 ** 6
+    with pytest.raises(ValueError):
+        case.cache.rows(1, slot)
