@@ -11,7 +11,9 @@
 // consumer warps take 16 positions of each page each (mma.sync m16n8k16: a
 // tcgen05 tile would be 128 rows for 16), with a running maximum and sum of
 // their own that are joined once a tile.  The weights are multiplied as a
-// high and a low half, so they lose nothing to the 16-bit V product.
+// high and a low half, to 16 bits in BF16 and 22 in FP16 (there down to 2^-25 of a
+// warp's largest, where the low half and then the weight leave the type's
+// range), because these calls have the cycles: HBM bounds them.
 //
 // Measured: 48 streams of 4000 to 16,000 positions, 32 q heads on 8 of 128,
 // FP16: 290 us, 6.7 TB/s, a plain copy's rate.  128 streams of 200 to 4096,

@@ -435,7 +435,8 @@ int hb_paged_status(const hb_page_pool *pool, int32_t *status, void *stream);
  * not see never reach it, whatever they hold (rows near infinities or NaN in V
  * are done once more, slowly; a row that sees a NaN score is NaN at once).  Scores, sums and the running maximum are
  * FP32; for the product with V the weights are rounded to the element type in
- * calls with long chunks, else kept to twice its bits; out is rounded once.
+ * calls with long chunks, else kept to twice its bits (in FP16 to no less than
+ * 2^-25 of the largest); out is rounded once.
  * out must not overlap q. */
 int hb_paged_attend(const hb_page_pool *pool, int layer, const hb_paged_rows *rows, const hb_paged_query *query,
                     void *stream);

@@ -300,3 +300,42 @@ def test_rows_of_missing_pages_are_refused():
     case.cache.lengths[slot] = 10 ** 6
     with pytest.raises(ValueError):
         case.cache.rows(1, slot)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("heads", [(4, 4, 64), (3, 3, 128)])
+def test_few_rows_keep_the_weights_low_halves(heads, dtype):
+    """V chosen so that each output nearly cancels: what the weights lose in
+    the product with V is then all there is to see.  The bound is
+    test_paged_kv.py's with the weights' error as two halves have it: u^2 A,
+    and in FP16 2^-25 of each |v| where the low half is below the normal range
+    (the sum of the weights is at least 1)."""
+    torch = _torch()
+    qh, kvh, d = heads
+    case = Case(heads, dtype, [1] * 16, [3] * 16, seed=49)
+    case.q *= 0.25
+    u = 2.0 ** -8 if dtype == "bfloat16" else 2.0 ** -11
+    pool = case.cache.pool
+    at = torch.arange(8, device="cuda")[None] ^ torch.arange(3, device="cuda")[:, None]  # [position, block]
+    want, tol = [], []
+    for b, slot in enumerate(case.slots_np):
+        page = pool[int(case.table_np[slot, 0]), 1, :, :, :, :3].view(kvh, 2, d // 64, 3, 8, 8)
+        index = at.view(1, 1, 1, 3, 8, 1).expand_as(page)
+        plain = lambda: torch.take_along_dim(page, index, 4).transpose(2, 3).reshape(kvh, 2, 3, d).double()  # noqa: E731, B023
+        k, v = plain().unbind(1)
+        q = case.q[b].double()
+        w = torch.softmax((k * q[:, None]).sum(-1) * d ** -0.5, 1)[..., None]
+        v[:, 2] = -(w[:, :2] * v[:, :2]).sum(1) / w[:, 2]
+        stored = v.to(case.dtype).reshape(kvh, 3, d // 64, 8, 8).transpose(1, 2)
+        page[:, 1] = torch.take_along_dim(stored, index[:, 1], 3)
+        v = plain()[:, 1]
+        o, a = (w * v).sum(1), (w * v.abs()).sum(1)
+        ds = (d + 8) * 2.0 ** -24 * (k.abs() * q[:, None].abs()).sum(-1).amax(1, keepdim=True) * d ** -0.5
+        want.append(o)
+        tol.append(u * o.abs() + (u * u + 2 * ds + 2.0 ** -18) * a + 2.0 ** -24
+                   + (2.0 ** -25 * v.abs().sum(1) if dtype == "float16" else 0))
+    out, _ = case.attend()
+    case.cache.status()
+    off = (out.double() - torch.stack(want)).abs() / torch.stack(tol)
+    assert float(off.max()) <= 1, float(off.max())
