@@ -108,6 +108,8 @@ int check_shape(const char *who, const hb_page_pool *p) {
   if (p->n_pages < 1 || p->layers < 1 || p->kv_heads < 1 || p->n_slots < 1 || p->table_width < 1 ||
       p->table_width > (1 << 24) || p->kv_heads > 1024 || p->layers > 4096)
     return fail(nullptr, HB_ERR_INVALID_ARG, "%s: pages, layers, kv heads, slots and table width must be positive", who);
+  if (static_cast<int64_t>(p->n_slots) * p->table_width > INT32_MAX)   // what a reserve's page counts can add up to
+    return fail(nullptr, HB_ERR_UNSUPPORTED, "%s: the table must have fewer than 2^31 entries", who);
   if (p->page_stride < layer_bytes(*p) * p->layers || p->page_stride % 128)
     return fail(nullptr, HB_ERR_INVALID_ARG, "%s: page_stride must be a multiple of 128 and hold a page", who);
   return HB_OK;
@@ -425,7 +427,7 @@ int hb_pages_free(const hb_page_pool *pool, int n, const int32_t *slots_dev, voi
   if (!slots_dev) return fail(nullptr, HB_ERR_INVALID_ARG, "hb_pages_free: null pointer");
   int sms = 0;
   if ((rc = device_info("hb_pages_free", &sms))) return rc;
-  HB_CUDA(nullptr, launch(pg::free_kernel, (n + 3) / 4, 128, 0, static_cast<cudaStream_t>(stream), pool_view(*pool), slots_dev, n));
+  HB_CUDA(nullptr, launch(pg::free_kernel, n / 4 + (n % 4 ? 1 : 0), 128, 0, static_cast<cudaStream_t>(stream), pool_view(*pool), slots_dev, n));
   return HB_OK;
 }
 

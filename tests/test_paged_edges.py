@@ -339,3 +339,19 @@ def test_few_rows_keep_the_weights_low_halves(heads, dtype):
     case.cache.status()
     off = (out.double() - torch.stack(want)).abs() / torch.stack(tol)
     assert float(off.max()) <= 1, float(off.max())
+
+
+def test_c_refusal_of_tables_past_32_bits():
+    """Page counts of a call are summed in 32 bits: over all slots they can
+    reach the table's entries."""
+    import ctypes
+
+    lib = hb_lib.load()
+    fake = 1 << 20
+    pool = dict(pages_dev=fake, page_stride=16384, n_pages=4, layers=1, kv_heads=1, head_dim=64, element=0,
+                table_dev=fake, refs_dev=fake, lengths_dev=fake, workspace_dev=fake, workspace_bytes=1 << 60)
+    make = lambda slots, width: ctypes.byref(hb_lib.HbPagePool(n_slots=slots, table_width=width, **pool))  # noqa: E731
+    assert lib.hb_paged_workspace_bytes(make(1 << 10, 1 << 20)) > 0
+    for slots, width in ((1 << 11, 1 << 20), (1 << 20, 1 << 12), (2 ** 31 - 1, 2)):
+        assert lib.hb_paged_workspace_bytes(make(slots, width)) == 0
+        assert lib.hb_pages_reserve(make(slots, width), 1, fake, fake, None) == hb_lib.HB_ERR_UNSUPPORTED
