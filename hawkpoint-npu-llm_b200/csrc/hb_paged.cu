@@ -199,10 +199,10 @@ int launch_copy(const hb_page_pool &p, void *to_pages, int to_n, const int *from
 // has the call alone if no entry has more than 8 of its tiles and the average
 // is at most 32 packed rows (heads of 64) or 8 (heads of 128).  Measured, rows
 // kernel alone / otherwise, us: heads of 64, 64 streams of 1024 with 21 packed
-// rows each 20.3 / 22.9, with 63 30.9 / 23.2; 96 streams of 200 to 2000 of which
-// 12 have 126 packed rows (21.9 on average) 25.6 / 34.2.  Heads of 128: 64 streams
-// with 24 packed rows 104 / 69; 96 streams, 12 with 32 (7.5 on average) 102 / 104,
-// 12 with 64 (11.5) 122 / 107.  All entries alike above that are the tiles
+// rows each 19.9 / 23.6, with 63 30.0 / 23.9; 96 streams of 200 to 2000 of which
+// 12 have 126 packed rows (21.9 on average) 25.3 / 35.8.  Heads of 128: 64 streams
+// with 24 packed rows 98 / 69; 96 streams, 12 with 32 (7.5 on average) 94 / 100,
+// 12 with 64 (11.5) 112 / 104.  All entries alike above that are the tiles
 // kernel's alone.  A bound on an entry's rows that is wrong costs time, not
 // rows: a kernel launched alone takes every entry.
 template <int D, class T>

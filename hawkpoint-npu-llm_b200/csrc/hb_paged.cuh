@@ -85,7 +85,7 @@ __device__ __forceinline__ void grid_begin() {
 
 // A call of two kernels, the second launched early and beside the first, whose
 // results it does not need, only what the first one's wait made visible.  A
-// wait of its own would last until the first one ends (7 to 12 us more in a
+// wait of its own would last until the first one ends (7 to 11 us more in a
 // step of 96 streams of which 12 or 24 have chunks).  So the first's first block
 // counts kFirst up when it has waited, before it lets the second begin, and
 // the second's blocks count one up each: a block that finds the first one's

@@ -20,7 +20,7 @@
 // A new page is always the lowest free one, so results do not depend on the
 // order threads run in.  Measured: a fork of one stream 7.4 us (two launches
 // and the books' four phases); of 64, 49 MB of partial pages copied, 18 us;
-// compaction of 1.1 GB 189 us, 5.9 TB/s of 6.5; free and reserve for 32
+// compaction of 1.1 GB 191 us, 5.9 TB/s of 6.5; free and reserve for 32
 // slots 8.4 us.  Books and copies as one launch, the blocks waiting for a
 // flag, cost 1.3 us less of the host and 3.1 us more on the device.
 #pragma once

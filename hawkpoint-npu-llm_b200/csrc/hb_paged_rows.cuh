@@ -15,10 +15,12 @@
 // warp's largest, where the low half and then the weight leave the type's
 // range), because these calls have the cycles: HBM bounds them.
 //
-// Measured: 48 streams of 4000 to 16,000 positions, 32 q heads on 8 of 128,
-// FP16: 290 us, 6.7 TB/s, a plain copy's rate.  128 streams of 200 to 4096,
+// Measured in replays of a CUDA graph over three sets of inputs (of the largest,
+// 2 GB a call, some pages are then still in L2): 48 streams of 4000 to 16,000
+// positions, 32 q heads on 8 of 128, FP16: 286 us; call by call, inputs anew,
+// 323 us, 6.1 TB/s, 93 % of a plain copy's rate.  128 streams of 200 to 4096,
 // 14 heads on 2 of 64, BF16: 33 us, 4.4 TB/s; 5 us to the first page's scores,
-// 22 of pages at a copy's rate, 2.7 of joins, the rest pieces of unlike length.
+// 22 of pages at a copy's rate, 2.7 of joins, the rest not accounted for.
 // One such stream of 4032: 9.9 us, all of it latency.
 #pragma once
 

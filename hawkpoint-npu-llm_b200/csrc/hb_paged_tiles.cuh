@@ -19,23 +19,31 @@
 // the stale maximum, so the result is the same), which after the first blocks
 // is almost never.
 //
-// Measured, BF16: four prompts of 3000 to 4096 positions, 14 q heads on 2 of
-// 64: 162 us, 588 TFLOP/s, 2.0 times the exponentials' 83 us; a step of both
-// halves takes 3,300 cycles, 2,050 of them the exponentials themselves, the
+// Measured, BF16, in replays of a CUDA graph: four prompts of 3000 to 4096
+// positions, 14 q heads on 2 of 64: 164 us, 581 TFLOP/s, 2.0 times the
+// exponentials' 83 us; a step of both halves takes 3,300 cycles, 2,050 of them the exponentials themselves, the
 // rest scores on their way from the MMA, their maximum, and the hand-over of
 // the turn.  Chunks of 200 to 512 rows of four prompts, 32 q heads on 8 of 128,
-// window 1024: 54 us, 485 TFLOP/s; a multiprocessor has some 12 steps of 3,900
+// window 1024: 55 us, 476 TFLOP/s; a multiprocessor has some 12 steps of 3,900
 // cycles there (P lies over S, so a half's next S waits for its P V), and the
 // start (7 us to the first scores) and the joins weigh as much as they do.
 //
 // Warps 0-3 and 4-7: the softmax of either half; warp 8: MMA issue; warp 9:
-// K and V; warps 10 and 11: the halves' q, a tile ahead.  One block a
+// K and V; warps 10 and 11: the halves' q, a tile ahead with heads of 64, with
+// heads of 128 (one buffer) once the tile's last scores are issued.  One block a
 // multiprocessor; the line of blocks is cut evenly (hb_paged.cuh), a tile cut
 // by a border is joined by the last of its pieces to get to its end, which
 // keeps its own part in TMEM (all parts through memory: chunks 65 us instead
-// of 58, prompts 172 instead of 165).  The weights are rounded to 16 bits for
-// the product with V, as the MMA wants them; their sum is of what they were
-// before, in FP32.
+// of 58, prompts 172 instead of 165).
+//
+// The weights are rounded once to the element type for the product with V, whose
+// operands have one type; their sum is of what they were before, in FP32.  The
+// output's error against 64 bits is 0.0020 to 0.0023 of its norm in BF16 and
+// 0.00025 to 0.00028 in FP16, where its own rounding alone gives 0.0016 and
+// 0.0002.  A low half beside the high one, as the rows kernel has it, would
+// come to those, at half as many MMAs more, 128 subtractions and 64 conversions
+// of pairs more a row and step in the softmax warps that bound the kernel, and
+// with heads of 64 no TMEM is left for it (S 256 columns, O 128, P 128).
 #pragma once
 
 #include "hb_paged_rows.cuh"

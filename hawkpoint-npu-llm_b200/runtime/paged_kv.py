@@ -208,7 +208,9 @@ class PagedKVCache:
         slots' positions up to each row's own (with ``window``: the last
         ``window`` of them); ``scale`` defaults to 1 / sqrt(head_dim).  Returns
         the output in q's shape; with ``lse`` also float32 [rows, q heads], the
-        log of the sum of exp(scores).  Rows that see nothing give 0 and -inf."""
+        log of the sum of exp(scores).  Rows that see nothing give 0 and -inf.
+        ``out`` must not overlap ``q``.  No gradient is recorded, whatever q
+        requires."""
         (rows, heads, d), (q_row, q_head, _) = self._heads("q", q)
         if out is None:
             out, o_row, o_head = self._new_heads(rows, heads), heads * d, d
