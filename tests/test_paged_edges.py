@@ -355,3 +355,45 @@ def test_c_refusal_of_tables_past_32_bits():
     for slots, width in ((1 << 11, 1 << 20), (1 << 20, 1 << 12), (2 ** 31 - 1, 2)):
         assert lib.hb_paged_workspace_bytes(make(slots, width)) == 0
         assert lib.hb_pages_reserve(make(slots, width), 1, fake, fake, None) == hb_lib.HB_ERR_UNSUPPORTED
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(14, 2, 64), (16, 2, 128)])
+def test_rows_of_no_entry_where_one_kernel_has_all_entries(heads):
+    """Entries alike, as max_rows says: whole chunks (201 x 3 rows of which 3
+    belong to none), then single tokens (2 x 3, 3 of none), and starts that descend."""
+    torch = _torch()
+    for rows, most in (([200, 200, 200], 201), ([1, 1, 1], 2)):
+        case = Case(heads, "bfloat16", rows, [250, 300, 400], seed=50)
+        want, want_lse = case.check()
+        n = case.n_rows
+        case.q = torch.cat([torch.randn_like(case.q[:2]), case.q, torch.randn_like(case.q[:1])])
+        case.row_start, case.max_rows = case.row_start + 2, most
+        out, lse = case.attend(out=torch.full_like(case.q, 7.0))
+        case.cache.status()
+        assert torch.equal(out[2: n + 2], want) and torch.equal(lse[2: n + 2], want_lse)
+        assert not bool(out[:2].any()) and not bool(out[-1].any())
+        assert bool((lse[:2] == -np.inf).all()) and bool((lse[-1] == -np.inf).all())
+        case.row_start = case.row_start[torch.tensor([0, 2, 1, 3], device="cuda")].contiguous()
+        out, lse = case.attend(out=torch.full_like(case.q, 7.0))
+        with pytest.raises(hb_lib.HbError, match="out of range"):
+            case.cache.status()
+        assert not bool(out.any()) and bool((lse == -np.inf).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (16, 2, 128)])
+def test_an_infinity_in_v_reaches_a_single_token(heads, dtype):
+    """Infinity in the dim that has it, whatever a weight's low half is; the other dims as without it."""
+    torch = _torch()
+    case = Case(heads, dtype, [1, 1], [300, 90], seed=51)
+    clean, lse = case.check()
+    poisoned(case, 150, 1, float("-inf"), dim=45)
+    out, same = case.attend()
+    case.cache.status()
+    assert bool((out[0, :, 45] == -np.inf).all()) and torch.equal(lse, same) and torch.equal(out[1], clean[1])
+    out[0, :, 45] = clean[0, :, 45]
+    _, _, tol, _ = case.reference()
+    tol[0, :, 45] = 1
+    assert bool(((out.double() - clean.double()).abs() <= 2 * tol).all())
