@@ -230,7 +230,11 @@ cudaError_t launch_attend(pg::Attend A, int max_rows, int sms, cudaStream_t st) 
   A.shape.extra = pg::kTilesExtra;
   A.arrived = A.arrived2;
   A.parts = A.parts2;
-  return launch(pg::paged_tiles_kernel<D, T>, sms, pg::kTilesThreads, pg::TilesSize<D>::kSmem + line, st, A, pg::kTilesLeast);
+  const cudaError_t err =
+      launch(pg::paged_tiles_kernel<D, T>, sms, pg::kTilesThreads, pg::TilesSize<D>::kSmem + line, st, A, pg::kTilesLeast);
+  // the rows kernel's count would be taken for the next call's
+  if (err != cudaSuccess && A.beside) cudaMemsetAsync(&A.pool.control->began, 0, sizeof(int), st);
+  return err;
 }
 
 template <int D, class T>

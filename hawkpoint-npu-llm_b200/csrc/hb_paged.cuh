@@ -77,7 +77,7 @@ __device__ __forceinline__ Entry entry_of(const Pool &P, const Batch &B, int b) 
 // Every kernel here is launched early (programmatic launch): its blocks take
 // their places while the kernel before it ends, wait for it and what it wrote,
 // and let the next one do the same.  Waiting comes first, so that at most two
-// kernels of a stream are under way (three where an attention call has two).
+// kernels of a stream are under way.
 __device__ __forceinline__ void grid_begin() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
